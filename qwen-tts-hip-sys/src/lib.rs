@@ -15,6 +15,10 @@ pub const QTTS_ERR_IO: c_int = -6;
 pub const QTTS_F32: c_int = 0;
 pub const QTTS_BF16: c_int = 1;
 
+pub const QTTS_KV_BF16: c_int = 0;
+pub const QTTS_KV_E4M3: c_int = 1;
+pub const QTTS_KV_INT8: c_int = 2;
+
 #[repr(C)]
 pub struct qtts_ctx {
     _p: [u8; 0],
@@ -91,6 +95,64 @@ pub struct qtts_gen_debug {
     pub shared_rng_stream: c_int,
     pub done_cb: qtts_done_cb,
     pub done_user: *mut c_void,
+}
+
+#[repr(C)]
+pub struct qtts_kv_cache {
+    _p: [u8; 0],
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct qtts_kv_config {
+    pub layers: c_int,
+    pub pages: c_int,
+    pub page_tokens: c_int,
+    pub kv_heads: c_int,
+    pub head_dim: c_int,
+    pub format: c_int,
+}
+
+/// The pointers of this and the next two structs are device memory.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct qtts_kv_batch {
+    pub n_seq: c_int,
+    pub n_tokens: c_int,
+    pub max_new: c_int,
+    pub max_ctx: c_int,
+    pub max_pages: c_int,
+    pub q_start: *const i32,
+    pub ctx_len: *const i32,
+    pub page_table: *const i32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct qtts_kv_rows {
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub dtype: c_int,
+    pub k_token_stride: i64,
+    pub k_head_stride: i64,
+    pub v_token_stride: i64,
+    pub v_head_stride: i64,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct qtts_kv_attend_args {
+    pub q: *const c_void,
+    pub out: *mut c_void,
+    pub q_token_stride: i64,
+    pub q_head_stride: i64,
+    pub out_token_stride: i64,
+    pub out_head_stride: i64,
+    pub n_heads: c_int,
+    pub scale: c_float,
+    pub window: c_int,
+    pub workspace: *mut c_void,
+    pub workspace_bytes: i64,
 }
 
 extern "C" {
@@ -259,6 +321,38 @@ extern "C" {
         B: c_int,
         frames_stride: c_int,
         emb_out: *mut c_float,
+    ) -> c_int;
+
+    pub fn qtts_kv_open(ctx: *mut qtts_ctx, cfg: *const qtts_kv_config, out: *mut *mut qtts_kv_cache) -> c_int;
+    pub fn qtts_kv_close(kv: *mut qtts_kv_cache);
+    pub fn qtts_kv_bytes(kv: *mut qtts_kv_cache) -> i64;
+    pub fn qtts_kv_write(
+        kv: *mut qtts_kv_cache,
+        layer: c_int,
+        batch: *const qtts_kv_batch,
+        rows: *const qtts_kv_rows,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn qtts_kv_read(
+        kv: *mut qtts_kv_cache,
+        layer: c_int,
+        batch: *const qtts_kv_batch,
+        rows: *const qtts_kv_rows,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn qtts_kv_attend_workspace(
+        kv: *mut qtts_kv_cache,
+        batch: *const qtts_kv_batch,
+        n_heads: c_int,
+        window: c_int,
+        bytes: *mut i64,
+    ) -> c_int;
+    pub fn qtts_kv_attend(
+        kv: *mut qtts_kv_cache,
+        layer: c_int,
+        batch: *const qtts_kv_batch,
+        args: *const qtts_kv_attend_args,
+        stream: *mut c_void,
     ) -> c_int;
 
     pub fn qtts_model_info(

@@ -9,6 +9,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libqtts_hip.so")
 
 QTTS_F32, QTTS_BF16 = 0, 1
+KV_FORMATS = {"bf16": 0, "e4m3": 1, "int8": 2}
 
 
 class QttsError(RuntimeError):
@@ -50,13 +51,35 @@ class GenDebug(C.Structure):
                 ("done_cb", DONE_CB), ("done_user", C.c_void_p)]
 
 
+class KvConfig(C.Structure):
+    _fields_ = [("layers", C.c_int), ("pages", C.c_int), ("page_tokens", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int),
+                ("format", C.c_int)]
+
+
+class KvBatch(C.Structure):
+    _fields_ = [("n_seq", C.c_int), ("n_tokens", C.c_int), ("max_new", C.c_int), ("max_ctx", C.c_int), ("max_pages", C.c_int),
+                ("q_start", C.c_void_p), ("ctx_len", C.c_void_p), ("page_table", C.c_void_p)]
+
+
+class KvRows(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int), ("k_token_stride", C.c_int64), ("k_head_stride", C.c_int64),
+                ("v_token_stride", C.c_int64), ("v_head_stride", C.c_int64)]
+
+
+class KvAttendArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64),
+                ("out_token_stride", C.c_int64), ("out_head_stride", C.c_int64), ("n_heads", C.c_int), ("scale", C.c_float),
+                ("window", C.c_int), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
 EXPORTS = ["qtts_init", "qtts_shutdown", "qtts_last_error", "qtts_stream", "qtts_model_create", "qtts_model_load_tensor",
            "qtts_model_load_tensor_device", "qtts_model_finalize", "qtts_model_load_dir", "qtts_model_free", "qtts_generate", "qtts_generate_ex",
            "qtts_last_timing", "qtts_codec_decode", "qtts_mel", "qtts_speaker_embed", "qtts_model_info",
            "qtts_gemm_profile", "qtts_bench_gemm", "qtts_bench_stream", "qtts_encode_audio",
            "qtts_speaker_embed_mel", "qtts_codec_stream_open", "qtts_codec_stream_push", "qtts_codec_stream_close",
            "qtts_mel_noalloc", "qtts_mel_noalloc_capacity", "qtts_session_open", "qtts_session_close", "qtts_session_stream",
-           "qtts_generate_continuous"]
+           "qtts_generate_continuous", "qtts_kv_open", "qtts_kv_close", "qtts_kv_bytes", "qtts_kv_write", "qtts_kv_read",
+           "qtts_kv_attend_workspace", "qtts_kv_attend"]
 
 _lib = None
 
@@ -109,6 +132,15 @@ def load():
     lib.qtts_gemm_profile.argtypes = [C.c_void_p, C.POINTER(C.c_double), C.c_int, C.POINTER(C.c_int)]
     lib.qtts_bench_gemm.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_double)]
     lib.qtts_bench_stream.argtypes = [C.c_void_p, C.c_long, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_double)]
+    lib.qtts_kv_open.argtypes = [C.c_void_p, C.POINTER(KvConfig), C.POINTER(C.c_void_p)]
+    lib.qtts_kv_close.argtypes = [C.c_void_p]
+    lib.qtts_kv_close.restype = None
+    lib.qtts_kv_bytes.argtypes = [C.c_void_p]
+    lib.qtts_kv_bytes.restype = C.c_int64
+    lib.qtts_kv_write.argtypes = [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]
+    lib.qtts_kv_read.argtypes = lib.qtts_kv_write.argtypes
+    lib.qtts_kv_attend_workspace.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.POINTER(C.c_int64)]
+    lib.qtts_kv_attend.argtypes = [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]
     _lib = lib
     return lib
 

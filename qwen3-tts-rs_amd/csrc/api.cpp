@@ -346,4 +346,43 @@ int qtts_model_info(qtts_model* m, int* hidden, int* vocab, int* groups, int* to
     QTTS_API_END
 }
 
+int qtts_kv_open(qtts_ctx* ctx, const qtts_kv_config* cfg, qtts_kv_cache** out) {
+    QTTS_API_BEGIN
+    QTTS_CHECK(ctx && cfg && out, ERR_BAD_ARG, "qtts_kv_open: null argument");
+    *out = reinterpret_cast<qtts_kv_cache*>(kv_open(&ctx->c, *cfg));
+    QTTS_API_END
+}
+
+void qtts_kv_close(qtts_kv_cache* kv) { kv_close(reinterpret_cast<KvCache*>(kv)); }
+
+int64_t qtts_kv_bytes(qtts_kv_cache* kv) { return kv ? kv_bytes(*reinterpret_cast<KvCache*>(kv)) : 0; }
+
+int qtts_kv_write(qtts_kv_cache* kv, int layer, const qtts_kv_batch* batch, const qtts_kv_rows* rows, void* stream) {
+    QTTS_API_BEGIN
+    QTTS_CHECK(kv && batch && rows, ERR_BAD_ARG, "qtts_kv_write: null argument");
+    kv_write(*reinterpret_cast<KvCache*>(kv), layer, *batch, *rows, (hipStream_t)stream);
+    QTTS_API_END
+}
+
+int qtts_kv_read(qtts_kv_cache* kv, int layer, const qtts_kv_batch* batch, const qtts_kv_rows* rows, void* stream) {
+    QTTS_API_BEGIN
+    QTTS_CHECK(kv && batch && rows, ERR_BAD_ARG, "qtts_kv_read: null argument");
+    kv_read(*reinterpret_cast<KvCache*>(kv), layer, *batch, *rows, (hipStream_t)stream);
+    QTTS_API_END
+}
+
+int qtts_kv_attend_workspace(qtts_kv_cache* kv, const qtts_kv_batch* batch, int n_heads, int window, int64_t* bytes) {
+    QTTS_API_BEGIN
+    QTTS_CHECK(kv && batch && bytes, ERR_BAD_ARG, "qtts_kv_attend_workspace: null argument");
+    *bytes = kv_attend_workspace(*reinterpret_cast<KvCache*>(kv), *batch, n_heads, window);
+    QTTS_API_END
+}
+
+int qtts_kv_attend(qtts_kv_cache* kv, int layer, const qtts_kv_batch* batch, const qtts_kv_attend_args* args, void* stream) {
+    QTTS_API_BEGIN
+    QTTS_CHECK(kv && batch && args, ERR_BAD_ARG, "qtts_kv_attend: null argument");
+    kv_attend(*reinterpret_cast<KvCache*>(kv), layer, *batch, *args, (hipStream_t)stream);
+    QTTS_API_END
+}
+
 }  // extern "C"

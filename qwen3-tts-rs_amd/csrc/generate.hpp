@@ -37,4 +37,14 @@ size_t mel_scratch_bytes();
 void run_speaker_embed(Model& m, const float* audio, const int* n_samples, int B, int max_samples, float* emb_out);
 void run_speaker_embed_mel(Model& m, const float* mel, const int* n_frames, int B, int frames_stride, float* emb_out);
 
+// key/value cache handle (kv.cpp)
+struct KvCache;
+KvCache* kv_open(Ctx* ctx, const qtts_kv_config& c);
+void kv_close(KvCache* k);
+int64_t kv_bytes(const KvCache& k);
+void kv_write(const KvCache& k, int layer, const qtts_kv_batch& b, const qtts_kv_rows& r, hipStream_t st);
+void kv_read(const KvCache& k, int layer, const qtts_kv_batch& b, const qtts_kv_rows& r, hipStream_t st);
+int64_t kv_attend_workspace(const KvCache& k, const qtts_kv_batch& b, int n_heads, int window);
+void kv_attend(const KvCache& k, int layer, const qtts_kv_batch& b, const qtts_kv_attend_args& r, hipStream_t st);
+
 }  // namespace qtts

@@ -1,0 +1,555 @@
+// Attention of new tokens over the paged 8- or 16-bit cache (gfx950): prompts, chunks that continue one, drafted tokens, single
+// tokens (the talker's decode step: qwen_tts/src/nn/attention/mod.rs:359-472).
+//
+//   o_ih = sum_j softmax_j(scale q_ih . k_jg) v_jg,   g = h / (heads per kv head),  j <= p_i, j > p_i - window
+//
+// A row is one query head of one new token; the rows of a sequence and kv head, in token order, are cut into tiles, so any number of
+// heads per kv head fills a tile.  Keys are walked once with the running maximum m and sum l of the softmax in f32:
+//   S^T = K Q^T   K rows are the A operand, the tile's queries the B operand, so a lane holds scores of one row only and the softmax
+//                 needs no more than one or two lane swaps;
+//   O^T = V^T P^T the score registers are the B operand as they stand once the keys of a matrix step are numbered in the order in
+//                 which the lanes hold them; V^T comes out of a row-major LDS image by transposing reads.
+// Rounding: K, V and Q enter exactly (bf16, or codes times a power of two).  P is rounded to bf16 for the second product, at most
+// 2^-9 relative per term, of the order of the output's own rounding; l is summed from the unrounded f32 values.
+// Key ranges of few rows are cut into parts (KvAttendPlan) whose (m, l, O) a second launch joins.
+// A masked key may hold anything: its score is replaced, and its V row meets the products as zero.  Where some rows of a tile see a key
+// and others do not, a non-finite V element is taken out of the products and added to the rows that see it one by one.
+#include "kv_device.hpp"
+
+#include <algorithm>
+
+namespace qtts {
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+template <typename F>
+__device__ __forceinline__ float kv_quad_rows(float v, F op) {  // over lanes r, r + 16, r + 32, r + 48, left in all of them
+    return fold_rows(fold_halves(v, op), op);
+}
+__device__ __forceinline__ float fmax2(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ float fadd2(float a, float b) { return a + b; }
+
+// four V rows x 16 columns, transposed: lane 4 q + p of a 16-lane group points at row q, columns 4 p ..; it receives column
+// (lane & 15) of the four rows
+__device__ __forceinline__ s16x4_t read_tr4(const u16* p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)p);
+}
+__device__ __forceinline__ bf16x8_t join8(s16x4_t a, s16x4_t b) {
+    return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+__device__ __forceinline__ bool bf16_pair_bad(unsigned w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
+__device__ __forceinline__ bool bf16x8_bad(uint4 w) { return bf16_pair_bad(w.x) || bf16_pair_bad(w.y) || bf16_pair_bad(w.z) || bf16_pair_bad(w.w); }
+__device__ __forceinline__ unsigned bf16_pair_clean(unsigned w) {
+    if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
+    if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
+    return w;
+}
+__device__ __forceinline__ uint4 bf16x8_clean(uint4 w) {
+    return make_uint4(bf16_pair_clean(w.x), bf16_pair_clean(w.y), bf16_pair_clean(w.z), bf16_pair_clean(w.w));
+}
+// value added to a row that sees a V element: the element if it is not finite (it was taken out of the products), else nothing
+__device__ __forceinline__ float bad_only(u16 b) { return (b & 0x7f80u) == 0x7f80u ? bf16_bits_to_f32(b) : 0.f; }
+
+// ---------------------------------------------------------------------------------------------- at most 16 rows a tile
+template <int FMT, int D>
+__global__ __launch_bounds__(256) void kv_attend_few_kernel(KvAttendArgs a) {
+    constexpr bool Q8 = FMT != KV_BF16;
+    constexpr int NJ = D / 32, NDT = D / 16;
+    constexpr int KLD = Q8 ? D / 64 : D / 32;          // 16-byte loads of a K row per lane
+    constexpr int EPP = Q8 ? 16 : 8, PPR = D / EPP;    // V: elements per 16-byte piece, pieces per row
+    constexpr int RPI = 64 / PPR, NV = 32 / RPI;       // rows a wave loads at once, loads per 32 rows
+    constexpr int LDV = D + 16;                        // rows of the V image 8 banks apart (modulo 64): its reads hit every bank once
+    constexpr int LDO = D + 4;
+    constexpr int VBYTES = 4 * 32 * LDV * 2, OBYTES = 4 * 16 * LDO * 4;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[VBYTES > OBYTES ? VBYTES : OBYTES];
+    __shared__ float pm[4][16], pl[4][16];
+
+    const int pair = blockIdx.x;
+    if (pair >= a.b.n_seq * a.kv.nkv) return;
+    const KvTile t = kv_tile<16>(a, pair, blockIdx.y, blockIdx.z);
+    if (!t.live) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, gq = lane >> 4;
+    u16* Vs = reinterpret_cast<u16*>(smem) + wave * 32 * LDV;
+
+    // this lane's row: its key range and its query
+    const int row = t.row0 + r;
+    const bool has = row < t.rows;
+    const int tok = (has ? row : t.row0) / t.G, head = t.g * t.G + (has ? row : t.row0) - tok * t.G;
+    const int pos = t.s.ctx - t.s.n + tok;
+    const int klo = has ? (a.window ? pos - a.window + 1 : 0) : 0x7fffffff;
+    bf16x8_t q[NJ];
+    {
+        const u16* qp = (const u16*)a.q + (long)(t.s.t0 + tok) * a.q_token_stride + (long)head * a.q_head_stride;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int d0 = Q8 ? 64 * (j >> 1) + 16 * gq + 8 * (j & 1) : 32 * j + 8 * gq;
+            q[j] = *reinterpret_cast<const bf16x8_t*>(qp + d0);
+        }
+    }
+
+    f32x4_t acc[NDT];
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) acc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    const float sc = a.scale * 1.4426950408889634f;  // exponentials to base 2
+
+    uint4 kreg[2][KLD], vreg[NV];
+    unsigned ksc[2], vsc[NV];
+    auto load = [&](int kb, const int (&pg)[2]) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            const size_t kr = kv_row(a.kv, max(pg[kt], 0), 0, t.g, kb + 16 * kt) + r;
+            const unsigned char* kp = a.kv.codes + kr * (Q8 ? D : 2 * D) + gq * 16;
+#pragma unroll
+            for (int j = 0; j < KLD; ++j) kreg[kt][j] = *reinterpret_cast<const uint4*>(kp + 64 * j);
+            if constexpr (Q8)
+                ksc[kt] = D == 128 ? *reinterpret_cast<const unsigned*>(a.kv.scales + kr * 4) : *reinterpret_cast<const u16*>(a.kv.scales + kr * 2);
+        }
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+            const int k0 = n * RPI;  // the wave's first row of this load; all of them in one group of 16
+            const size_t vr = kv_row(a.kv, max(pg[k0 >> 4], 0), 1, t.g, kb + k0) + lane / PPR;
+            vreg[n] = *reinterpret_cast<const uint4*>(a.kv.codes + vr * (Q8 ? D : 2 * D) + (lane % PPR) * 16);
+            if constexpr (Q8) vsc[n] = a.kv.scales[vr * (D / KV_BLOCK) + (lane % PPR) / 2];
+        }
+    };
+
+    int kb = t.s0 + wave * 32;
+    int pg[2] = {kv_page16(a, t, kb), kv_page16(a, t, kb + 16)};
+    if (kb < t.s1) load(kb, pg);
+    int pn[2] = {kv_page16(a, t, kb + 128), kv_page16(a, t, kb + 144)};
+    for (; kb < t.s1; kb += 128) {
+        // V rows into this wave's image: rows outside the tile's range and holes as zeros
+        const bool mixed = t.p0 != t.p1 && (kb + 31 > t.p0 || (a.window && kb <= t.p1 - a.window));
+        uint4 w[NV][Q8 ? 2 : 1];
+        bool bad = false;
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+            const int key = kb + n * RPI + lane / PPR;
+            const bool in = key >= t.k_begin && key < t.s1 && pg[(n * RPI) >> 4] >= 0;
+            if constexpr (Q8) {
+                const float f = kv_scale(vsc[n]);
+                w[n][0] = kv_decode8<FMT>(make_uint2(vreg[n].x, vreg[n].y), f);
+                w[n][1] = kv_decode8<FMT>(make_uint2(vreg[n].z, vreg[n].w), f);
+            } else {
+                w[n][0] = vreg[n];
+            }
+#pragma unroll
+            for (int h = 0; h < (Q8 ? 2 : 1); ++h) {
+                if (!in) w[n][h] = make_uint4(0u, 0u, 0u, 0u);
+                if (mixed) bad |= bf16x8_bad(w[n][h]);
+                *reinterpret_cast<uint4*>(Vs + (n * RPI + lane / PPR) * LDV + (lane % PPR) * EPP + 8 * h) = w[n][h];
+            }
+        }
+        // scores of 2 x 16 keys: s[kt][i] = key kb + 16 kt + 4 gq + i
+        f32x4_t s[2];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            s[kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            if constexpr (Q8) {
+#pragma unroll
+                for (int j = 0; j < KLD; ++j) {
+                    const float f = kv_scale((ksc[kt] >> (8 * (2 * j + (gq >> 1)))) & 0xffu);
+                    const uint4 c = kreg[kt][j];
+                    s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kv_decode8<FMT>(make_uint2(c.x, c.y), f)), q[2 * j], s[kt], 0, 0, 0);
+                    s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kv_decode8<FMT>(make_uint2(c.z, c.w), f)), q[2 * j + 1], s[kt], 0, 0, 0);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < KLD; ++j)
+                    s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kreg[kt][j]), q[j], s[kt], 0, 0, 0);
+            }
+        }
+        // the next rows travel while these go through the softmax
+        const int pc[2] = {pg[0], pg[1]};
+        pg[0] = pn[0];
+        pg[1] = pn[1];
+        if (kb + 128 < t.s1) load(kb + 128, pg);
+        pn[0] = kv_page16(a, t, kb + 256);
+        pn[1] = kv_page16(a, t, kb + 272);
+
+        float p[8], mx = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int key = kb + 16 * (e >> 2) + 4 * gq + (e & 3);
+            const bool see = key >= klo && key <= pos && key < t.s1 && pc[e >> 2] >= 0;
+            p[e] = see ? s[e >> 2][e & 3] * sc : -INFINITY;
+            mx = fmaxf(mx, p[e]);
+        }
+        const float mn = fmaxf(m, kv_quad_rows(mx, fmax2));
+        const float ref = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: every exponential below is 0
+        const float alpha = __builtin_amdgcn_exp2f(m - ref);
+        m = mn;
+        float ps = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            p[e] = __builtin_amdgcn_exp2f(p[e] - ref);
+            ps += p[e];
+        }
+        l = l * alpha + ps;
+        const bf16x8_t ph = __builtin_bit_cast(bf16x8_t, make_uint4(pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]), pack_bf16(p[4], p[5]), pack_bf16(p[6], p[7])));
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) acc[dt] *= alpha;
+        __builtin_amdgcn_wave_barrier();  // the image is this wave's own: its LDS accesses are served in order
+        if (mixed && __any(bad)) {
+            for (int j = 0; j < 32; ++j) {
+                const int key = kb + j;
+                if (key >= klo && key <= pos && has) {
+#pragma unroll
+                    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[dt][i] += bad_only(Vs[j * LDV + 16 * dt + 4 * gq + i]);
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int n = 0; n < NV; ++n)
+#pragma unroll
+                for (int h = 0; h < (Q8 ? 2 : 1); ++h)
+                    *reinterpret_cast<uint4*>(Vs + (n * RPI + lane / PPR) * LDV + (lane % PPR) * EPP + 8 * h) = bf16x8_clean(w[n][h]);
+            __builtin_amdgcn_wave_barrier();
+        }
+        const u16* vrow = Vs + (4 * gq + (r >> 2)) * LDV + 4 * (r & 3);
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) {
+            const bf16x8_t vt = join8(read_tr4(vrow + 16 * dt), read_tr4(vrow + 16 * LDV + 16 * dt));
+            acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt, ph, acc[dt], 0, 0, 0);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+
+    // join the four waves
+    l = kv_quad_rows(l, fadd2);
+    __syncthreads();
+    float* Os = reinterpret_cast<float*>(smem);
+    if (gq == 0) {
+        pm[wave][r] = m;
+        pl[wave][r] = l;
+    }
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) *reinterpret_cast<f32x4_t*>(Os + (wave * 16 + r) * LDO + 16 * dt + 4 * gq) = acc[dt];
+    __syncthreads();
+    constexpr int EPT = D / 16;
+    const int orow = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * EPT;
+    if (t.row0 + orow >= t.rows) return;
+    float M = pm[0][orow];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) M = fmaxf(M, pm[w][orow]);
+    float L = 0.f, o[EPT];
+#pragma unroll
+    for (int e = 0; e < EPT; ++e) o[e] = 0.f;
+    const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float wt = __builtin_amdgcn_exp2f(pm[w][orow] - ref);
+        L += wt * pl[w][orow];
+#pragma unroll
+        for (int e = 0; e < EPT; ++e) o[e] += wt * Os[(w * 16 + orow) * LDO + d0 + e];
+    }
+    if (t.parts > 1) {
+        const size_t u = ((size_t)(pair * a.tiles + blockIdx.y) * a.splits + blockIdx.z) * 16 + orow;
+        float* po = a.ws + u * D + d0;
+#pragma unroll
+        for (int e = 0; e < EPT; e += 4) *reinterpret_cast<float4*>(po + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        if ((threadIdx.x & 15) == 0) {
+            float* ml = a.ws + (size_t)a.b.n_seq * a.kv.nkv * a.tiles * a.splits * 16 * D + u * 2;
+            ml[0] = M;
+            ml[1] = L;
+        }
+        return;
+    }
+    const int rr = t.row0 + orow, tk = rr / t.G, hd = t.g * t.G + rr - tk * t.G;
+    bf16_t* op = (bf16_t*)a.out + (long)(t.s.t0 + tk) * a.out_token_stride + (long)hd * a.out_head_stride + d0;
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+    for (int e = 0; e < EPT; e += 4) {
+        const float v[4] = {o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv};
+        store4_split(op + e, a.out_lo, v);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------ 128 rows a tile
+template <int FMT, int D>
+__global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) {
+    constexpr bool Q8 = FMT != KV_BF16;
+    constexpr int KB = 64;
+    constexpr int NS = D / 16, NDT = D / 32;          // contraction steps of K Q^T; 32-column tiles of the output
+    constexpr int EPP = Q8 ? 16 : 8, PPR = D / EPP;   // elements per 16-byte piece of the cache, pieces per row
+    constexpr int KPW = 64 / PPR, NP = KB / (4 * KPW);  // keys a wave stages at once, passes per block of keys
+    constexpr int LDK = D + 8;    // K rows 4 banks apart: 16 lanes' 16-byte reads hit every bank once
+    constexpr int LDV = D + 32;   // V rows 16 banks apart (modulo 64): the four rows of a transposing read share no bank
+    __shared__ __attribute__((aligned(16))) u16 Ks[KB * LDK];
+    __shared__ __attribute__((aligned(16))) u16 Vs[KB * LDV];
+    __shared__ int sh_bad;
+
+    const int pair = blockIdx.x;
+    if (pair >= a.b.n_seq * a.kv.nkv) return;
+    const int tile = (int)gridDim.y - 1 - (int)blockIdx.y;  // the last tiles see the most keys: they start first
+    const KvTile t = kv_tile<128>(a, pair, tile, blockIdx.z);
+    if (!t.live) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 31, hf = lane >> 5;
+    const int wrow0 = t.row0 + wave * 32;
+    const bool wlive = wrow0 < t.rows;
+    const int first = t.s.ctx - t.s.n;
+    const int wp0 = first + min(wrow0, t.rows - 1) / t.G, wp1 = first + min(wrow0 + 31, t.rows - 1) / t.G;
+
+    const int row = wrow0 + r;
+    const bool has = row < t.rows;
+    const int rr = has ? row : t.rows - 1;
+    const int tok = rr / t.G, head = t.g * t.G + rr - tok * t.G;
+    const int pos = first + tok;
+    const int klo = has ? (a.window ? pos - a.window + 1 : 0) : 0x7fffffff;
+    bf16x8_t q[NS];
+    {
+        const u16* qp = (const u16*)a.q + (long)(t.s.t0 + tok) * a.q_token_stride + (long)head * a.q_head_stride + 8 * hf;
+#pragma unroll
+        for (int j = 0; j < NS; ++j) q[j] = *reinterpret_cast<const bf16x8_t*>(qp + 16 * j);
+    }
+    f32x16_t acc[NDT];
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    const float sc = a.scale * 1.4426950408889634f;
+
+    uint4 kreg[NP], vreg[NP];
+    unsigned ksc[NP], vsc[NP];
+    const int krow = lane / PPR, pc = lane % PPR;
+    auto load = [&](int kb, const int (&pg)[4]) {
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            const int k0 = (n * 4 + wave) * KPW;  // the wave's first key of this pass; all of them in one group of 16
+            const size_t kr = kv_row(a.kv, max(pg[k0 >> 4], 0), 0, t.g, kb + k0) + krow;
+            const size_t vr = kr + ((size_t)a.kv.nkv << a.kv.page_shift);
+            kreg[n] = *reinterpret_cast<const uint4*>(a.kv.codes + kr * (Q8 ? D : 2 * D) + pc * 16);
+            vreg[n] = *reinterpret_cast<const uint4*>(a.kv.codes + vr * (Q8 ? D : 2 * D) + pc * 16);
+            if constexpr (Q8) {
+                ksc[n] = a.kv.scales[kr * (D / KV_BLOCK) + pc / 2];
+                vsc[n] = a.kv.scales[vr * (D / KV_BLOCK) + pc / 2];
+            }
+        }
+    };
+    auto pages = [&](int kb, int (&pg)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pg[i] = kv_page16(a, t, kb + 16 * i);
+    };
+
+    int pg[4], pn[4];
+    pages(t.s0, pg);
+    if (t.s0 < t.s1) load(t.s0, pg);
+    pages(t.s0 + KB, pn);
+    if (threadIdx.x == 0) sh_bad = -1;
+    for (int kb = t.s0; kb < t.s1; kb += KB) {
+        const bool mixed = kb + KB - 1 > t.p0 || (a.window && kb <= t.p1 - a.window);
+        uint4 w[NP][Q8 ? 2 : 1];
+        __syncthreads();  // every wave is done with the previous image
+        bool bad = false;
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            const int k0 = (n * 4 + wave) * KPW;
+            const int key = k0 + krow;
+            const bool in = kb + key >= t.k_begin && kb + key < t.s1 && pg[k0 >> 4] >= 0;
+            if constexpr (Q8) {
+                const float fk = kv_scale(ksc[n]), fv = kv_scale(vsc[n]);
+                *reinterpret_cast<uint4*>(Ks + key * LDK + pc * 16) = kv_decode8<FMT>(make_uint2(kreg[n].x, kreg[n].y), fk);
+                *reinterpret_cast<uint4*>(Ks + key * LDK + pc * 16 + 8) = kv_decode8<FMT>(make_uint2(kreg[n].z, kreg[n].w), fk);
+                w[n][0] = kv_decode8<FMT>(make_uint2(vreg[n].x, vreg[n].y), fv);
+                w[n][1] = kv_decode8<FMT>(make_uint2(vreg[n].z, vreg[n].w), fv);
+            } else {
+                *reinterpret_cast<uint4*>(Ks + key * LDK + pc * 8) = kreg[n];
+                w[n][0] = vreg[n];
+            }
+#pragma unroll
+            for (int h = 0; h < (Q8 ? 2 : 1); ++h) {
+                if (!in) w[n][h] = make_uint4(0u, 0u, 0u, 0u);
+                if (mixed) bad |= bf16x8_bad(w[n][h]);
+                *reinterpret_cast<uint4*>(Vs + key * LDV + pc * EPP + 8 * h) = w[n][h];
+            }
+        }
+        if (bad) sh_bad = kb;
+        int pcur[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { pcur[i] = pg[i]; pg[i] = pn[i]; }
+        if (kb + KB < t.s1) load(kb + KB, pg);
+        pages(kb + 2 * KB, pn);
+        __syncthreads();
+        if (mixed && sh_bad == kb) {
+            if (wlive) {
+                for (int j = 0; j < KB; ++j) {
+                    const int key = kb + j;
+                    if (key >= klo && key <= pos) {
+#pragma unroll
+                        for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) acc[dt][i] += bad_only(Vs[j * LDV + 32 * dt + 8 * (i >> 2) + 4 * hf + (i & 3)]);
+                    }
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int n = 0; n < NP; ++n)
+#pragma unroll
+                for (int h = 0; h < (Q8 ? 2 : 1); ++h)
+                    *reinterpret_cast<uint4*>(Vs + ((n * 4 + wave) * KPW + krow) * LDV + pc * EPP + 8 * h) = bf16x8_clean(w[n][h]);
+            __syncthreads();
+        }
+        // wave-uniform: no row of this wave sees the block
+        if (!wlive || kb > wp1 || (a.window && kb + KB <= wp0 - a.window + 1)) continue;
+
+        f32x16_t s[2];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[kt][i] = 0.f;
+            const u16* kp = Ks + (kt * 32 + r) * LDK + 8 * hf;
+#pragma unroll
+            for (int j = 0; j < NS; ++j)
+                s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8_t*>(kp + 16 * j), q[j], s[kt], 0, 0, 0);
+        }
+        // s[kt][i] = key kb + 32 kt + 8 (i / 4) + 4 hf + i % 4 of this lane's row
+        const bool whole = kb + KB - 1 <= wp0 && !(a.window && kb <= wp1 - a.window) && kb + KB <= t.s1 && pcur[0] >= 0 && pcur[1] >= 0 && pcur[2] >= 0 && pcur[3] >= 0;
+        if (!whole) {
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int key = kb + 32 * kt + 8 * (i >> 2) + 4 * hf + (i & 3);
+                    const bool see = key >= klo && key <= pos && key < t.s1 && pcur[2 * kt + (i >> 3)] >= 0;
+                    s[kt][i] = see ? s[kt][i] : -INFINITY;
+                }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kt][i] * sc);
+        mx = fold_halves(mx, fmax2);
+        const float mn = fmaxf(m, mx);
+        const float ref = mn == -INFINITY ? 0.f : mn;
+        if (__any(mn > m)) {
+            const float alpha = __builtin_amdgcn_exp2f(m - ref);
+            l *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) acc[dt] *= alpha;
+            m = mn;
+        }
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                float p[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][8 * u + e], sc, -ref));
+                    l += p[e];
+                }
+                const bf16x8_t ph = __builtin_bit_cast(bf16x8_t, make_uint4(pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]), pack_bf16(p[4], p[5]), pack_bf16(p[6], p[7])));
+                const u16* vrow = Vs + (32 * kt + 16 * u + 4 * hf + ((lane & 15) >> 2)) * LDV + (lane & 16) + 4 * (lane & 3);
+#pragma unroll
+                for (int dt = 0; dt < NDT; ++dt)
+                    acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(join8(read_tr4(vrow + 32 * dt), read_tr4(vrow + 8 * LDV + 32 * dt)), ph, acc[dt], 0, 0, 0);
+            }
+    }
+
+    l = fold_halves(l, fadd2);
+    if (!has) return;
+    if (t.parts > 1) {
+        const size_t u = ((size_t)(pair * a.tiles + tile) * a.splits + blockIdx.z) * 128 + wave * 32 + r;
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<float4*>(a.ws + u * D + 32 * dt + 2 * i + 4 * hf) = make_float4(acc[dt][i], acc[dt][i + 1], acc[dt][i + 2], acc[dt][i + 3]);
+        if (hf == 0) {
+            float* ml = a.ws + (size_t)a.b.n_seq * a.kv.nkv * a.tiles * a.splits * 128 * D + u * 2;
+            ml[0] = m;
+            ml[1] = l;
+        }
+        return;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    bf16_t* op = (bf16_t*)a.out + (long)(t.s.t0 + tok) * a.out_token_stride + (long)head * a.out_head_stride + 4 * hf;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const float v[4] = {acc[dt][i] * inv, acc[dt][i + 1] * inv, acc[dt][i + 2] * inv, acc[dt][i + 3] * inv};
+            store4_split(op + 32 * dt + 2 * i, a.out_lo, v);
+        }
+}
+
+// ------------------------------------------------------------------------------------------------ joining the parts
+template <int TR, int D>
+__global__ __launch_bounds__(256) void kv_attend_join_kernel(KvAttendArgs a) {
+    constexpr int EPT = D / 16;
+    const int unit = blockIdx.x, pair = unit / a.tiles, tile = unit - pair * a.tiles;
+    const KvTile t = kv_tile<TR>(a, pair, tile, 0);
+    const int orow = blockIdx.y * 16 + (threadIdx.x >> 4), d0 = (threadIdx.x & 15) * EPT;
+    const int rr = t.row0 + orow;
+    if (!t.live || t.parts == 1 || rr >= t.rows) return;
+    const size_t u = (size_t)unit * a.splits * TR + orow;
+    const float* ml = a.ws + (size_t)a.b.n_seq * a.kv.nkv * a.tiles * a.splits * TR * D + u * 2;
+    const float* po = a.ws + u * D + d0;
+    float M = -INFINITY;
+    for (int s = 0; s < t.parts; ++s) M = fmaxf(M, ml[(size_t)s * TR * 2]);
+    const float ref = M == -INFINITY ? 0.f : M;
+    float L = 0.f, o[EPT];
+#pragma unroll
+    for (int e = 0; e < EPT; ++e) o[e] = 0.f;
+    for (int s = 0; s < t.parts; ++s) {
+        const float wt = __builtin_amdgcn_exp2f(ml[(size_t)s * TR * 2] - ref);
+        L += wt * ml[(size_t)s * TR * 2 + 1];
+#pragma unroll
+        for (int e = 0; e < EPT; e += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(po + (size_t)s * TR * D + e);
+            o[e] += wt * v.x;
+            o[e + 1] += wt * v.y;
+            o[e + 2] += wt * v.z;
+            o[e + 3] += wt * v.w;
+        }
+    }
+    const int tk = rr / t.G, hd = t.g * t.G + rr - tk * t.G;
+    bf16_t* op = (bf16_t*)a.out + (long)(t.s.t0 + tk) * a.out_token_stride + (long)hd * a.out_head_stride + d0;
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+    for (int e = 0; e < EPT; e += 4) {
+        const float v[4] = {o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv};
+        store4_split(op + e, a.out_lo, v);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------- host side
+void launch_kv_attend(hipStream_t st, KvAttendArgs a, const KvAttendPlan& p) {
+    if (a.b.n_seq == 0 || a.b.n_tokens == 0) return;
+    QTTS_CHECK(p.splits == 1 || a.ws, ERR_BAD_ARG, "kv attend: workspace missing");
+    a.tiles = p.tiles;
+    a.splits = p.splits;
+    a.split_len = p.split_len;
+    const unsigned pairs = (unsigned)(a.b.n_seq * a.kv.nkv);
+    // pairs vary fastest and are padded to the number of XCDs: all tiles and parts of a pair run on one XCD and share its L2
+    const dim3 grid((pairs + 7) / 8 * 8, (unsigned)p.tiles, (unsigned)p.splits), join(pairs * (unsigned)p.tiles, (unsigned)(p.tile_rows / 16));
+#define QTTS_KV_ATTEND(FMT, DD)                                                                        \
+    if (a.kv.format == FMT && a.kv.d == DD) {                                                          \
+        if (p.tile_rows == 16) kv_launch(kv_attend_few_kernel<FMT, DD>, grid, dim3(256), st, a);       \
+        else kv_launch(kv_attend_tile_kernel<FMT, DD>, grid, dim3(256), st, a);                        \
+        if (p.splits > 1) {                                                                            \
+            if (p.tile_rows == 16) kv_launch(kv_attend_join_kernel<16, DD>, join, dim3(256), st, a);   \
+            else kv_launch(kv_attend_join_kernel<128, DD>, join, dim3(256), st, a);                    \
+        }                                                                                              \
+        return;                                                                                        \
+    }
+    QTTS_KV_ATTEND(KV_BF16, 64)
+    QTTS_KV_ATTEND(KV_E4M3, 64)
+    QTTS_KV_ATTEND(KV_INT8, 64)
+    QTTS_KV_ATTEND(KV_BF16, 128)
+    QTTS_KV_ATTEND(KV_E4M3, 128)
+    QTTS_KV_ATTEND(KV_INT8, 128)
+#undef QTTS_KV_ATTEND
+    throw Error(ERR_SHAPE, "kv cache: head_dim must be 64 or 128");
+}
+
+}  // namespace qtts

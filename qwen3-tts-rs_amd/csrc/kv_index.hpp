@@ -1,0 +1,102 @@
+// Where the kernels of the paged cache read and write: lengths, pages and key ranges out of a batch's arrays.  Compiled for the host
+// too, so that a test on the CPU can show that nothing these arrays hold leads outside a buffer.
+#pragma once
+#include "kv.hpp"
+
+#include <algorithm>
+
+#define QTTS_KV_HD __host__ __device__ __forceinline__
+
+namespace qtts {
+
+QTTS_KV_HD int kv_min(int a, int b) { return a < b ? a : b; }
+QTTS_KV_HD int kv_max(int a, int b) { return a > b ? a : b; }
+QTTS_KV_HD int kv_clamp(int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); }
+
+// New tokens [t0, t0 + n) and context length of sequence s.  Lengths come from device memory, where the host cannot check
+// them: they are cut to the bounds that the launch was checked for, so that no access leaves a buffer whatever they hold.
+struct KvSeq {
+    int t0, n, ctx, row;
+};
+QTTS_KV_HD KvSeq kv_seq(const KvBatch& b, int s) {
+    KvSeq q;
+    int t0 = s, t1 = s + 1;
+    if (b.q_start) {
+        t0 = b.q_start[s];
+        t1 = b.q_start[s + 1];
+    }
+    q.t0 = kv_clamp(t0, 0, b.n_tokens);
+    q.n = kv_clamp(kv_clamp(t1, q.t0, b.n_tokens) - q.t0, 0, b.max_new);
+    q.ctx = kv_clamp(b.ctx_len[(long)s * b.ctx_stride], 0, b.max_ctx);
+    q.row = b.rows ? b.rows[s] : s;
+    return q;
+}
+// physical page of a position, -1 = hole
+QTTS_KV_HD int kv_page(const KvLayer& kv, int row, int pos) {
+    const long i = (long)row * kv.max_pages + (pos >> kv.page_shift);
+    if (!kv.page_table) return (int)i;
+    const int p = kv.page_table[i];
+    return (unsigned)p < (unsigned)kv.n_pages ? p : -1;
+}
+// index of a head row within the layer (its elements start at index * d, its scales at index * d / 32)
+QTTS_KV_HD size_t kv_row(const KvLayer& kv, int page, int which, int g, int pos) {
+    return (((((size_t)page * 2 + which) * kv.nkv + g)) << kv.page_shift) + (pos & ((1 << kv.page_shift) - 1));
+}
+
+// What a block works on: tile `tile` of TR rows of sequence and kv head `pair`, part `part` of its keys.
+struct KvTile {
+    KvSeq s;
+    int g, G, rows;         // rows of the sequence and kv head in all
+    int row0;               // first row of the tile
+    int p0, p1;             // positions of its first and last token
+    int k_begin, k_end;     // keys any of its rows can see
+    int s0, s1, parts;      // keys of this part; parts with keys
+    bool live;
+};
+template <int TR>
+QTTS_KV_HD KvTile kv_tile(const KvAttendArgs& a, int pair, int tile, int part) {
+    KvTile t;
+    t.live = false;
+    const int b = pair / a.kv.nkv;
+    t.g = pair - b * a.kv.nkv;
+    t.s = kv_seq(a.b, b);
+    t.G = a.nh / a.kv.nkv;
+    t.rows = t.s.n * t.G;
+    t.row0 = tile * TR;
+    if (t.row0 >= t.rows) return t;
+    const int first = t.s.ctx - t.s.n;  // negative where the caller claims more new tokens than the sequence has: those see nothing
+    t.p0 = first + t.row0 / t.G;
+    t.p1 = first + kv_min(t.row0 + TR - 1, t.rows - 1) / t.G;
+    t.k_begin = a.window ? kv_max(0, t.p0 - a.window + 1) : 0;
+    t.k_end = t.p1 + 1;
+    const int base = t.k_begin & ~63;
+    t.parts = kv_max(1, (t.k_end - base + a.split_len - 1) / a.split_len);
+    t.s0 = base + part * a.split_len;
+    t.s1 = kv_min(t.s0 + a.split_len, t.k_end);
+    t.live = part < t.parts;
+    return t;
+}
+// page of the 16 keys from `key` on, -1 = hole or past the part; key is a multiple of 16 and the same in every lane
+QTTS_KV_HD int kv_page16(const KvAttendArgs& a, const KvTile& t, int key) {
+    return key < t.s1 ? kv_page(a.kv, t.s.row, key) : -1;
+}
+
+// ---- host
+inline KvAttendPlan kv_attend_plan(const KvLayer& kv, const KvBatch& b, int nh, int window) {
+    KvAttendPlan p{};
+    const long rows = (long)b.max_new * (nh / kv.nkv);
+    p.tile_rows = rows <= 64 ? 16 : 128;
+    p.tiles = (int)std::min<long>((rows + p.tile_rows - 1) / p.tile_rows, 65536);  // the grid's y: callers refuse more than 65535
+    // keys the tile with the most of them can see
+    const long span_tokens = std::min<long>(b.max_new, (p.tile_rows - 1) / (nh / kv.nkv) + 2);
+    const long keys = std::max<long>(1, window ? std::min<long>(b.max_ctx, window + span_tokens + 63) : b.max_ctx);
+    const long units = (long)b.n_seq * kv.nkv * p.tiles;
+    const long want = std::max<long>(1, 1024 / std::max<long>(units, 1));
+    const long most = std::max<long>(1, (keys + 511) / 512);
+    p.splits = (int)std::min<long>(std::min(want, most), 256);
+    p.split_len = (int)(((keys + p.splits - 1) / p.splits + 127) / 128 * 128);
+    if (p.splits > 1) p.ws_bytes = (size_t)units * p.splits * p.tile_rows * (kv.d + 2) * sizeof(float);
+    return p;
+}
+
+}  // namespace qtts
