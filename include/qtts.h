@@ -55,6 +55,10 @@ int qtts_model_load_tensor(qtts_model* m, const char* hf_key, const void* data, 
 /* Same, with `data` already resident in this GPU's memory (synthetic benchmarks; no reference counterpart). */
 int qtts_model_load_tensor_device(qtts_model* m, const char* hf_key, const void* data, int src_dtype,
                                   const int64_t* shape, int rank);
+/* Holds the talker's key/value cache in the format QTTS_KV_E4M3 or QTTS_KV_INT8 (defined with qtts_kv_open below): half the
+ * memory and half the bytes a decode step reads per key.  QTTS_KV_BF16, the default, keeps it in the model's dtype.  bf16 models
+ * only.  Takes effect with the next generate call on the handle; sessions opened later start with the model's choice. */
+int qtts_model_set_kv_cache(qtts_model* m, int format);
 /* Checks that every tensor the configs require is present, builds fused weights, RoPE tables and the
  * normalised codebooks (audio/quantizer.rs:56-59). */
 int qtts_model_finalize(qtts_model* m);

@@ -132,6 +132,7 @@ struct AttnShape {
 struct KVCacheLayer {
     std::vector<float> k, v;  // [nkv][cap][d]
     int len = 0, cap = 0;
+    float top = 0.f;  // > 0: keys and values are held in 8 bits (448: e4m3, 127: int8; see hold8 in oracle_tts.cpp)
 };
 
 struct RopeTable {  // rope/core.rs:150-160 + rope/standard.rs:72-97 / rope/talker.rs:67-92
@@ -146,6 +147,7 @@ enum MaskMode { MASK_NONE = 0, MASK_CAUSAL = 1 };
 // One pre-norm decoder layer over T new tokens at positions pos0..pos0+T-1 with KV cache
 // (nn/decoder_layer.rs:63-86, nn/attention/unified.rs:179-243, nn/attention/mod.rs:359-472,
 // nn/mlp.rs:59-82).  x is [T][hidden], updated in place.
+void set_kv_hold(float top);  // 8-bit format of the talker's cache in the generate calls that follow (KVCacheLayer::top)
 void set_round_probe(int mask);  // diagnostic: see oracle_tts.cpp
 void probe_round(float* x, size_t n, int bit);
 void decoder_layer(const Weights& w, const std::string& prefix, const AttnShape& a, const RopeTable& rope,

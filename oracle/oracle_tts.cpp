@@ -207,6 +207,25 @@ void RopeTable::cos_sin(int64_t pos, float* c, float* s) const {
     }
 }
 
+// What a head row is held as in an 8-bit cache: blocks of 32 elements with a scale 2^e, e the smallest integer >= -100 with
+// max |x| <= top 2^e; x 2^-e rounded to nearest even, to an integer (top 127) or to three mantissa bits with a smallest step of 2^-9 (top 448).
+static float g_kv_top = 0.f;
+void set_kv_hold(float top) { g_kv_top = top; }
+static void hold8(float* x, int d, float top) {
+    for (int b = 0; b < d; b += 32) {
+        double a = 0;
+        for (int i = 0; i < 32; ++i) a = std::max(a, std::fabs((double)x[b + i]));
+        int e = -100;
+        while (a > std::ldexp((double)top, e)) ++e;
+        for (int i = 0; i < 32; ++i) {
+            const double y = std::ldexp((double)x[b + i], -e);
+            double step = 1.0;
+            if (top != 127.f) step = std::ldexp(1.0, std::max(y == 0 ? -6 : std::ilogb(y), -6) - 3);
+            x[b + i] = (float)std::ldexp(std::nearbyint(y / step) * step, e);
+        }
+    }
+}
+
 // -------------------------------------------------------------------------- decoder layer
 // Diagnostic only (0 in every parity check): rounds the named intermediate tensors to bf16 so that the storage precision of
 // a reduced-precision implementation can be priced tensor by tensor.  bit 0: normed layer inputs, bit 1: keys / values,
@@ -261,6 +280,10 @@ void decoder_layer(const Weights& w, const std::string& p, const AttnShape& a, c
         for (int h = 0; h < nkv; ++h) {
             std::memcpy(&cache.k[((size_t)h * cache.cap + cache.len + t) * d], &k[((size_t)t * nkv + h) * d], sizeof(float) * d);
             std::memcpy(&cache.v[((size_t)h * cache.cap + cache.len + t) * d], &v[((size_t)t * nkv + h) * d], sizeof(float) * d);
+            if (cache.top > 0.f) {
+                hold8(&cache.k[((size_t)h * cache.cap + cache.len + t) * d], d, cache.top);
+                hold8(&cache.v[((size_t)h * cache.cap + cache.len + t) * d], d, cache.top);
+            }
         }
     const int kv_len = cache.len + T;
     const int rep = nh / nkv;
@@ -533,6 +556,7 @@ void Model::generate(const GenRequest& r, const SamplingConfig& s_in, int max_ne
     std::vector<KVCacheLayer> cache((size_t)cfg.talker.layers);
     for (auto& c : cache) {
         c.cap = P + max_new_tokens + 1;
+        c.top = g_kv_top;
         c.k.assign((size_t)cfg.talker.nkv * c.cap * cfg.talker.d, 0.f);
         c.v.assign((size_t)cfg.talker.nkv * c.cap * cfg.talker.d, 0.f);
     }

@@ -168,6 +168,7 @@ extern "C" {
         dtype: c_int,
         out: *mut *mut qtts_model,
     ) -> c_int;
+    pub fn qtts_model_set_kv_cache(m: *mut qtts_model, format: c_int) -> c_int;
     pub fn qtts_model_load_tensor(
         m: *mut qtts_model,
         hf_key: *const c_char,

@@ -78,7 +78,7 @@ EXPORTS = ["qtts_init", "qtts_shutdown", "qtts_last_error", "qtts_stream", "qtts
            "qtts_gemm_profile", "qtts_bench_gemm", "qtts_bench_stream", "qtts_encode_audio",
            "qtts_speaker_embed_mel", "qtts_codec_stream_open", "qtts_codec_stream_push", "qtts_codec_stream_close",
            "qtts_mel_noalloc", "qtts_mel_noalloc_capacity", "qtts_session_open", "qtts_session_close", "qtts_session_stream",
-           "qtts_generate_continuous", "qtts_kv_open", "qtts_kv_close", "qtts_kv_bytes", "qtts_kv_write", "qtts_kv_read",
+           "qtts_generate_continuous", "qtts_model_set_kv_cache", "qtts_kv_open", "qtts_kv_close", "qtts_kv_bytes", "qtts_kv_write", "qtts_kv_read",
            "qtts_kv_attend_workspace", "qtts_kv_attend"]
 
 _lib = None
@@ -132,6 +132,7 @@ def load():
     lib.qtts_gemm_profile.argtypes = [C.c_void_p, C.POINTER(C.c_double), C.c_int, C.POINTER(C.c_int)]
     lib.qtts_bench_gemm.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_double)]
     lib.qtts_bench_stream.argtypes = [C.c_void_p, C.c_long, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_double)]
+    lib.qtts_model_set_kv_cache.argtypes = [C.c_void_p, C.c_int]
     lib.qtts_kv_open.argtypes = [C.c_void_p, C.POINTER(KvConfig), C.POINTER(C.c_void_p)]
     lib.qtts_kv_close.argtypes = [C.c_void_p]
     lib.qtts_kv_close.restype = None

@@ -113,6 +113,13 @@ int qtts_model_create(qtts_ctx* ctx, const char* config_json, const char* codec_
     QTTS_API_END
 }
 
+int qtts_model_set_kv_cache(qtts_model* m, int format) {
+    QTTS_API_BEGIN
+    QTTS_CHECK(m, ERR_BAD_ARG, "qtts_model_set_kv_cache: null model");
+    m->m.set_kv_cache(format);
+    QTTS_API_END
+}
+
 int qtts_model_load_tensor(qtts_model* m, const char* hf_key, const void* data, int src_dtype, const int64_t* shape, int rank) {
     QTTS_API_BEGIN
     QTTS_CHECK(m && hf_key && shape, ERR_BAD_ARG, "qtts_model_load_tensor: null argument");

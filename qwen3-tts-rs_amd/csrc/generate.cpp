@@ -13,6 +13,8 @@
 #include "runner.hpp"
 
 #include <algorithm>
+#include <array>
+#include <cstddef>
 #include <chrono>
 #include <cmath>
 #include <cstring>
@@ -78,6 +80,7 @@ struct GenState {
     DevBuf row_len, step, eos_step, active, row_max, hist, uniforms, codes, trailing_len, tts_pad;
     DevBuf trace_logits, trace_hidden, trace_cp;
     StackRun talker, cp;
+    DevBuf kv8_codes, kv8_scales, kv8_ws, kv8_runs;  // the talker's cache in 8 bits, its attention's workspace, the runs of a prompt launch
     size_t cap_rows = 0;
     GemmTimer timer;                         // optional HIP-event timing of every GEMM launch
     DevBuf icl;                              // reference code ids + destination rows of ICL prompts
@@ -317,12 +320,32 @@ static void generate_impl(Model& m, const qtts_request* reqs, int n, const qtts_
     m.ensure_rope(m.cp, G + 2);
 
     // KV pools
+    KvStack kv8;  // used when m.kv_format asks for an 8-bit cache
+    static_assert(offsetof(Tok, pos) == sizeof(int), "kv8.batch takes a token's position from its second integer");
     {
         const int max_pages = (max_ctx + PAGE_TOKENS - 1) / PAGE_TOKENS;
         // every row owns max_pages consecutive pages: no page table, no dependent load in front of the K/V accesses
         const size_t page_elems = (size_t)2 * c.talker.nkv * PAGE_TOKENS * c.talker.d;
         const size_t npages = (size_t)B * max_pages;
-        g.talker.pool.ensure((size_t)c.talker.layers * npages * page_elems * es);
+        if (m.kv_format == KV_BF16) {
+            g.talker.pool.ensure((size_t)c.talker.layers * npages * page_elems * es);
+            g.kv8_codes.release();
+            g.kv8_scales.release();
+        } else {
+            g.talker.pool.release();
+            const size_t head_rows = npages * (size_t)2 * c.talker.nkv * PAGE_TOKENS;
+            g.kv8_codes.ensure((size_t)c.talker.layers * head_rows * c.talker.d);
+            g.kv8_scales.ensure((size_t)c.talker.layers * head_rows * (c.talker.d / KV_BLOCK));
+            kv8.base = KvLayer{g.kv8_codes.as<unsigned char>(), g.kv8_scales.as<unsigned char>(), m.kv_format, c.talker.nkv, c.talker.d,
+                               __builtin_ctz(PAGE_TOKENS), (int)npages, max_pages, nullptr};
+            kv8.layer_rows = head_rows;
+            // decode steps: token b is row b's newest
+            const int tiles = (c.talker.nh / c.talker.nkv + 15) / 16, parts = (max_pages * PAGE_TOKENS + KV_TALKER_PART - 1) / KV_TALKER_PART;
+            kv8.batch = KvBatch{B, B, 1, max_pages * PAGE_TOKENS, nullptr, reinterpret_cast<const int*>(g.toks_dec.as<Tok>()) + 1, (int)(sizeof(Tok) / sizeof(int)), 1, nullptr};
+            kv8.plan = KvAttendPlan{16, tiles, parts, KV_TALKER_PART, (size_t)B * c.talker.nkv * tiles * parts * 16 * (c.talker.d + 2) * sizeof(float)};
+            if (parts > 1) g.kv8_ws.ensure(kv8.plan.ws_bytes);
+            kv8.ws = g.kv8_ws.as<float>();
+        }
         g.talker.kv = KVView{g.talker.pool.p, npages * page_elems, PAGE_TOKENS, c.talker.nkv, c.talker.d, max_pages, nullptr};
         QTTS_CHECK(G + 1 <= CP_PAGE_TOKENS, ERR_SHAPE, "generate: too many code groups for the code-predictor KV page");
         const size_t cpage = (size_t)2 * c.cp.nkv * CP_PAGE_TOKENS * c.cp.d;
@@ -477,6 +500,33 @@ static void generate_impl(Model& m, const qtts_request* reqs, int n, const qtts_
             launch_gather_rows(st, g.text_rows.p, F32, d_trail + (size_t)i * Tt_max, g.trailing.as<float>() + (size_t)rws[(size_t)i] * Tt_max * H, F32,
                                Tt_max, H, H);
         QTTS_HIP(hipMemcpyAsync(g.tts_pad.p, g.text_rows.as<float>() + (size_t)2 * H, (size_t)H * 4, hipMemcpyDeviceToDevice, st));
+        // prompt launches over an 8-bit cache: every chunk's runs of one row as the sequences of a batch
+        std::vector<int> runs;
+        std::vector<std::array<int, 3>> run_off;  // offset, sequences, longest run
+        if (m.kv_format != KV_BF16) {
+            for (int o = 0; o < Ttot; o += chunk_rows) {
+                build_attn_tiles(pl.p_toks.data() + o, std::min(chunk_rows, Ttot - o), ctiles);
+                std::vector<int> start, len, rows_of;
+                for (const AttnTile& t : ctiles) {  // neighbouring tiles that continue each other are one run
+                    const Tok& first = pl.p_toks[(size_t)(o + t.m0)];
+                    const Tok& last = pl.p_toks[(size_t)(o + t.m0 + t.count - 1)];
+                    if (!rows_of.empty() && rows_of.back() == t.row && len.back() == first.pos) {
+                        len.back() = last.pos + 1;
+                        continue;
+                    }
+                    start.push_back(t.m0);
+                    rows_of.push_back(t.row);
+                    len.push_back(last.pos + 1);
+                }
+                start.push_back(std::min(chunk_rows, Ttot - o));
+                int longest = 0;
+                for (size_t i = 0; i + 1 < start.size(); ++i) longest = std::max(longest, start[i + 1] - start[i]);
+                run_off.push_back({(int)runs.size(), (int)len.size(), longest});
+                for (const auto* v : {&start, &len, &rows_of}) runs.insert(runs.end(), v->begin(), v->end());
+            }
+            g.kv8_runs.ensure(runs.size() * 4);
+            copy_sync(g.kv8_runs.p, runs.data(), runs.size() * 4, hipMemcpyHostToDevice, st);
+        }
         // prefill (generation.rs:884-903)
         std::vector<int> last_src, last_dst;
         int row_end = 0;
@@ -491,7 +541,17 @@ static void generate_impl(Model& m, const qtts_request* reqs, int n, const qtts_
             // final norm output reuses act (T) and q (f32) as scratch rows
             R.tiles = g.tiles_prompt.as<AttnTile>() + ptile_off[(size_t)(o / chunk_rows)];
             R.n_tiles = (int)(ptile_off[(size_t)(o / chunk_rows) + 1] - ptile_off[(size_t)(o / chunk_rows)]);
+            KvStack kvp = kv8;
+            if (m.kv_format != KV_BF16) {
+                const auto& ro = run_off[(size_t)(o / chunk_rows)];
+                const int* d = g.kv8_runs.as<int>() + ro[0];
+                kvp.batch = KvBatch{ro[1], M, ro[2], kv8.batch.max_ctx, d, d + ro[1] + 1, 1, 0, d + 2 * ro[1] + 1};
+                const int tiles = (int)(((long)ro[2] * (c.talker.nh / c.talker.nkv) + 127) / 128);
+                kvp.plan = KvAttendPlan{128, tiles, 1, (kv8.batch.max_ctx + 127) & ~127, 0};
+                R.kv8 = &kvp;
+            }
             R.stack(m.talker, M, g.toks_prompt.as<Tok>() + o, g.talker.kv, g.ws.act.p, g.ws.q.as<float>(), true, false, g.ws.lo_act);
+            R.kv8 = nullptr;
             R.tiles = nullptr;  // the code predictor's two-token prefill keeps the per-token kernel
             R.n_tiles = 0;
             last_src.clear();
@@ -791,7 +851,9 @@ static void generate_impl(Model& m, const qtts_request* reqs, int n, const qtts_
     };
     auto talker_step = [&]() {  // generation.rs:1002-1026
         launch_make_decode_toks(st, g.row_len.as<int>(), g.toks_dec.as<Tok>(), B, c.talker.window, g.active.as<int>());
+        R.kv8 = m.kv_format != KV_BF16 ? &kv8 : nullptr;
         R.stack(m.talker, B, g.toks_dec.as<Tok>(), g.talker.kv, hid_t, hid_f, true, true, lo_cp);
+        R.kv8 = nullptr;  // the code predictor's contexts are short: they stay in the model's dtype
     };
     auto trace_copy = [&](int step) {
         // logits of this frame are recomputed into the partial buffer by frame_tail; hidden is in hid_f

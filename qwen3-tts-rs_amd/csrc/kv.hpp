@@ -35,7 +35,7 @@ struct KvBatch {
     int max_new, max_ctx;   // bounds on a sequence's new tokens and on ctx_len; what exceeds them is cut by the kernels
     const int* q_start;     // [n_seq + 1]; null: one new token per sequence
     const int* ctx_len;
-    int ctx_stride;         // elements between the sequences' ctx_len
+    int ctx_stride, ctx_add;  // sequence b's length is ctx_len[b ctx_stride] + ctx_add
     const int* rows;        // page-table row of each sequence, null: sequence b has row b
 };
 
@@ -79,6 +79,24 @@ struct KvAttendPlan {
 void launch_kv_attend(hipStream_t st, KvAttendArgs a, const KvAttendPlan& p);
 
 // one launch with its error as an exception (hipGetLastError would also report what other code left there)
+// The talker's cache in 8 bits (generate.cpp): rows that own consecutive pages, as KVView without a table, and the batch of the
+// launch at hand.  The plan does not depend on what else is in the batch: single tokens in parts of KV_TALKER_PART keys, prompts in
+// tiles with all of their keys, so that a row's result is the same whatever rows it shares a launch with.
+constexpr int KV_TALKER_PART = 512;
+struct KvStack {
+    KvLayer base{};
+    size_t layer_rows = 0;  // head rows of a layer
+    KvBatch batch{};
+    KvAttendPlan plan{};
+    float* ws = nullptr;
+    KvLayer layer(int l) const {
+        KvLayer k = base;
+        k.codes += (size_t)l * layer_rows * base.d;
+        k.scales += (size_t)l * layer_rows * (base.d / KV_BLOCK);
+        return k;
+    }
+};
+
 template <typename A>
 void kv_launch(void (*kernel)(A), dim3 grid, dim3 block, hipStream_t st, A args) {
     void* p[] = {&args};

@@ -27,7 +27,7 @@ QTTS_KV_HD KvSeq kv_seq(const KvBatch& b, int s) {
     }
     q.t0 = kv_clamp(t0, 0, b.n_tokens);
     q.n = kv_clamp(kv_clamp(t1, q.t0, b.n_tokens) - q.t0, 0, b.max_new);
-    q.ctx = kv_clamp(b.ctx_len[(long)s * b.ctx_stride], 0, b.max_ctx);
+    q.ctx = kv_clamp(b.ctx_len[(long)s * b.ctx_stride] + b.ctx_add, 0, b.max_ctx);
     q.row = b.rows ? b.rows[s] : s;
     return q;
 }

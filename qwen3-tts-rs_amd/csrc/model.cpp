@@ -332,6 +332,15 @@ static void stack_view(const StackW& b, StackW& v) {
     v.max_pos = 0;  // RoPE tables are grown on demand by the stream that needs them: each stream has its own
 }
 
+void Model::set_kv_cache(int format) {
+    QTTS_CHECK(format == KV_BF16 || format == KV_E4M3 || format == KV_INT8, ERR_BAD_ARG, "kv cache: format must be QTTS_KV_BF16, QTTS_KV_E4M3 or QTTS_KV_INT8");
+    if (format != KV_BF16) {
+        QTTS_CHECK(dtype == BF16, ERR_BAD_ARG, "kv cache: an 8-bit cache needs a bf16 model");
+        QTTS_CHECK(cfg.talker.d == 64 || cfg.talker.d == 128, ERR_SHAPE, "kv cache: an 8-bit cache needs a talker head_dim of 64 or 128");
+    }
+    kv_format = format;
+}
+
 void Model::init_view(const Model& base) {
     QTTS_CHECK(base.finalized, ERR_STATE, "session: the model is not finalized");
     QTTS_CHECK(!finalized && raw.empty(), ERR_STATE, "session: the handle already holds a model");
@@ -342,6 +351,7 @@ void Model::init_view(const Model& base) {
     tuning = base.tuning;
     tuning->latch(TUNE_SHARED);  // a session is opened: unless its first generate call came earlier, this weight set decodes with the kernels picked for several streams
     dtype = base.dtype;
+    kv_format = base.kv_format;
     cfg = base.cfg;
     codec = base.codec;
     stack_view(base.talker, talker);

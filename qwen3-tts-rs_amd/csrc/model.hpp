@@ -11,6 +11,7 @@
 #include "common.hpp"
 #include "json_min.hpp"
 #include "kernels.hpp"
+#include "kv.hpp"
 
 namespace qtts {
 
@@ -163,6 +164,7 @@ struct Model {
     std::shared_ptr<CpMemo> cp_memo = std::make_shared<CpMemo>();
     std::shared_ptr<Tuning> tuning = std::make_shared<Tuning>();
     int dtype = BF16;
+    int kv_format = KV_BF16;  // of the talker's cache; KV_BF16 = the model's dtype
     ModelCfg cfg;
     CodecCfg codec;
     bool finalized = false;
@@ -188,6 +190,7 @@ struct Model {
     void parse_config(const std::string& config_json, const char* codec_json);
     void load_tensor(const std::string& key, const void* data, int src_dtype, const int64_t* shape, int rank, bool on_device);
     void finalize();
+    void set_kv_cache(int format);
     const Tensor& get(const std::string& key) const;
     bool has(const std::string& key) const { return raw.count(key) != 0; }
     const float* f32(const std::string& key) const;

@@ -87,6 +87,8 @@ struct Runner {
     // (device array, build_attn_tiles) send their attention through the matrix-core tile kernel; null = one block per token
     const AttnTile* tiles = nullptr;
     int n_tiles = 0;
+    // set: the stack's keys and values are held in 8 bits there instead of in the KVView (the talker's launches)
+    const KvStack* kv8 = nullptr;
     Model& m;
     Workspace& g;
     GemmTimer* timer;
@@ -181,7 +183,9 @@ struct Runner {
         qa.q_norm = w.q_norm; qa.k_norm = w.k_norm; qa.eps = c.eps; qa.cos = s.cos.as<float>(); qa.sin = s.sin.as<float>();
         qa.rope_mode = 0; qa.toks = toks; qa.M = M; qa.nh = c.nh; qa.nkv = c.nkv; qa.d = c.d; qa.layer = kv_layer;
         qa.q_out = g.q.as<float>(); qa.uni_len = decode ? uni_len : 0; qa.small = tune_shared ? 1 : 0;
-        if (decode) {
+        if (kv8) {
+            attention_kv8(c, qa, kv_layer, (float)std::pow((double)c.d, -0.5));
+        } else if (decode) {
             launch_attention_decode(st, dt, qa, kv, (float)std::pow((double)c.d, -0.5), g.attn.p, lo_attn);
         } else {
             launch_qkv_post(st, dt, qa, kv);
@@ -231,6 +235,18 @@ struct Runner {
             launch_attention_tiles(st, dt, g.q.as<float>(), toks, tiles, n_tiles, kv, kv_layer, c.nh, scale, g.attn.p, lo_attn);
         else
             launch_attention(st, dt, g.q.as<float>(), toks, kv, kv_layer, M, c.nh, scale, g.attn.p, lo_attn);
+    }
+    // the same over the 8-bit cache, prompts and decode steps alike; the f32 query buffer takes the queries in bf16
+    void attention_kv8(const StackCfg& c, const QkvPostArgs& qa, int kv_layer, float scale) {
+        KvAttendArgs a{};
+        a.kv = kv8->layer(kv_layer);
+        launch_kv_qkv_post(st, qa, a.kv, g.q.p);
+        a.b = kv8->batch;
+        a.q = g.q.p; a.q_token_stride = (long)c.nh * c.d; a.q_head_stride = c.d;
+        a.out = g.attn.p; a.out_token_stride = (long)c.nh * c.d; a.out_head_stride = c.d; a.out_lo = lo_attn;
+        a.nh = c.nh; a.scale = scale; a.window = c.window >= a.b.max_ctx ? 0 : c.window;
+        a.ws = kv8->ws;
+        launch_kv_attend(st, a, kv8->plan);
     }
     // QTTS_PARTIAL_NORM=0: residual + RMSNorm passes of the decode layers as one block per row again
     static bool partial_norm_enabled() {

@@ -148,6 +148,7 @@ class LoaderConfig:  # model/loader.rs:31-54
     load_tokenizer: bool = True
     load_text_tokenizer: bool = True
     device: int = 0
+    kv_cache: Optional[str] = None  # format of the talker's key/value cache: None = dtype, "e4m3" or "int8" = 8 bits (bf16 models)
     load_encoder: bool = True   # codec encoder tensors (`encoder.*`): needed only for encode_audio / ICL voice clone
 
 
@@ -166,6 +167,8 @@ class Model:
         self._m = C.c_void_p()
         cj = json.dumps(codec_config).encode() if codec_config is not None else None
         check(self.lib.qtts_model_create(self._ctx, json.dumps(config).encode(), cj, self.dtype, C.byref(self._m)))
+        if loader.kv_cache is not None:
+            self.set_kv_cache(loader.kv_cache)
         self._finalized = False
         self.last_timing = None
         self.text_processor = None  # text.TextProcessor; set by ModelLoader when the directory holds tokenizer.json
@@ -228,6 +231,13 @@ class Model:
             src = QTTS_F32
         shape = (C.c_int64 * a.ndim)(*a.shape)
         check(self.lib.qtts_model_load_tensor(self._m, key.encode(), a.ctypes.data_as(C.c_void_p), src, shape, a.ndim))
+
+    def set_kv_cache(self, format: Optional[str]):
+        """Format of the talker's key/value cache from the next generate call on: None = the model's dtype, "e4m3" or "int8"
+        (qtts_model_set_kv_cache)."""
+        if format is not None and format not in ("e4m3", "int8"):
+            raise QttsError(-1, f"Unknown key/value cache format '{format}'. Available: [None, 'e4m3', 'int8']")
+        check(self.lib.qtts_model_set_kv_cache(self._m, _lib.KV_FORMATS[format or "bf16"]))
 
     def load_weights(self, items: Iterable):
         for k, a in items:
@@ -729,6 +739,8 @@ class ModelLoader:
         check(m.lib.qtts_model_load_dir(m._ctx, os.fsencode(self.model_dir), m.dtype, 1 if loader.load_tokenizer else 0,
                                         1 if loader.load_encoder else 0, C.byref(m._m)))
         m._finalized = True
+        if loader.kv_cache is not None:
+            m.set_kv_cache(loader.kv_cache)
         if loader.load_text_tokenizer and os.path.exists(os.path.join(self.model_dir, "tokenizer.json")):
             from .text import TextProcessor
             m.text_processor = TextProcessor.from_pretrained(self.model_dir)
@@ -736,11 +748,11 @@ class ModelLoader:
 
 
 def synthetic_model(shape: str, dtype: str = "bf16", seed: int = 20261111, model_type: str = "custom_voice", codec: bool = True,
-                    talker: bool = True, device: int = 0, round_to_bf16: bool = False, encoder: bool = False):
+                    talker: bool = True, device: int = 0, round_to_bf16: bool = False, encoder: bool = False, kv_cache: Optional[str] = None):
     """Random-init model of a named shape set (see synth.py).  Returns (Model, config, codec_config, template)."""
     from . import synth
     cfg, ccfg, tmpl = synth.shape_set(shape, model_type)
-    m = Model(cfg, ccfg if codec else None, LoaderConfig(dtype=dtype, device=device))
+    m = Model(cfg, ccfg if codec else None, LoaderConfig(dtype=dtype, device=device, kv_cache=kv_cache))
     keys = []
     if talker:
         keys += synth.talker_keys(cfg) + synth.speaker_keys(cfg)

@@ -56,7 +56,7 @@ int main() {
         for (int& x : ctx) x = any(max_pages << shift);
         for (int& x : table) x = any(a.kv.n_pages);
         a.kv.page_table = table.data();
-        a.b = KvBatch{n, in(1, 40), in(1, 40), in(0, max_pages << shift), start.data(), ctx.data(), 1, nullptr};
+        a.b = KvBatch{n, in(1, 40), in(1, 40), in(0, max_pages << shift), start.data(), ctx.data(), 1, 0, nullptr};
         a.nh = a.kv.nkv * in(1, 9);
         a.window = in(0, 2) ? 0 : in(1, 100);
         const KvAttendPlan p = kv_attend_plan(a.kv, a.b, a.nh, a.window);
