@@ -80,7 +80,7 @@ struct GenState {
     DevBuf row_len, step, eos_step, active, row_max, hist, uniforms, codes, trailing_len, tts_pad;
     DevBuf trace_logits, trace_hidden, trace_cp;
     StackRun talker, cp;
-    DevBuf kv8_codes, kv8_scales, kv8_ws, kv8_runs;  // the talker's cache in 8 bits, its attention's workspace, the runs of a prompt launch
+    DevBuf kv8_codes, kv8_scales, kv8_pages, kv8_ws, kv8_runs;  // the talker's cache in 8 bits, its attention's workspace, the runs of a prompt launch
     size_t cap_rows = 0;
     GemmTimer timer;                         // optional HIP-event timing of every GEMM launch
     DevBuf icl;                              // reference code ids + destination rows of ICL prompts
@@ -338,6 +338,11 @@ static void generate_impl(Model& m, const qtts_request* reqs, int n, const qtts_
             g.kv8_scales.ensure((size_t)c.talker.layers * head_rows * (c.talker.d / KV_BLOCK));
             kv8.base = KvLayer{g.kv8_codes.as<unsigned char>(), g.kv8_scales.as<unsigned char>(), m.kv_format, c.talker.nkv, c.talker.d,
                                __builtin_ctz(PAGE_TOKENS), (int)npages, max_pages, nullptr};
+            std::vector<int> own(npages);  // row r owns pages r max_pages .. r max_pages + max_pages - 1
+            for (size_t i = 0; i < npages; ++i) own[i] = (int)i;
+            g.kv8_pages.ensure(npages * 4);
+            copy_sync(g.kv8_pages.p, own.data(), npages * 4, hipMemcpyHostToDevice, st);
+            kv8.base.page_table = g.kv8_pages.as<int>();
             kv8.layer_rows = head_rows;
             // decode steps: token b is row b's newest
             const int tiles = (c.talker.nh / c.talker.nkv + 15) / 16, parts = (max_pages * PAGE_TOKENS + KV_TALKER_PART - 1) / KV_TALKER_PART;

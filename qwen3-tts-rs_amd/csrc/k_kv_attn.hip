@@ -38,16 +38,17 @@ __device__ __forceinline__ s16x4_t read_tr4(const u16* p) {
 __device__ __forceinline__ bf16x8_t join8(s16x4_t a, s16x4_t b) {
     return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
-__device__ __forceinline__ bool bf16_pair_bad(unsigned w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
-__device__ __forceinline__ bool bf16x8_bad(uint4 w) { return bf16_pair_bad(w.x) || bf16_pair_bad(w.y) || bf16_pair_bad(w.z) || bf16_pair_bad(w.w); }
+__device__ __forceinline__ bool bf16_pair_bad(unsigned w) { return ((w & 0x7f80u) == 0x7f80u) | ((w & 0x7f800000u) == 0x7f800000u); }
+__device__ __forceinline__ bool bf16x8_bad(u32x4_t w) { return bf16_pair_bad(w.x) | bf16_pair_bad(w.y) | bf16_pair_bad(w.z) | bf16_pair_bad(w.w); }
 __device__ __forceinline__ unsigned bf16_pair_clean(unsigned w) {
     if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
     if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
     return w;
 }
-__device__ __forceinline__ uint4 bf16x8_clean(uint4 w) {
-    return make_uint4(bf16_pair_clean(w.x), bf16_pair_clean(w.y), bf16_pair_clean(w.z), bf16_pair_clean(w.w));
+__device__ __forceinline__ u32x4_t bf16x8_clean(u32x4_t w) {
+    return u32x4_t{bf16_pair_clean(w.x), bf16_pair_clean(w.y), bf16_pair_clean(w.z), bf16_pair_clean(w.w)};
 }
+__device__ __forceinline__ u32x4_t keep(u32x4_t w, bool in) { return in ? w : u32x4_t{0u, 0u, 0u, 0u}; }
 // value added to a row that sees a V element: the element if it is not finite (it was taken out of the products), else nothing
 __device__ __forceinline__ float bad_only(u16 b) { return (b & 0x7f80u) == 0x7f80u ? bf16_bits_to_f32(b) : 0.f; }
 
@@ -95,7 +96,7 @@ __global__ __launch_bounds__(256) void kv_attend_few_kernel(KvAttendArgs a) {
     float m = -INFINITY, l = 0.f;
     const float sc = a.scale * 1.4426950408889634f;  // exponentials to base 2
 
-    uint4 kreg[2][KLD], vreg[NV];
+    u32x4_t kreg[2][KLD], vreg[NV];
     unsigned ksc[2], vsc[NV];
     auto load = [&](int kb, const int (&pg)[2]) {
 #pragma unroll
@@ -103,7 +104,7 @@ __global__ __launch_bounds__(256) void kv_attend_few_kernel(KvAttendArgs a) {
             const size_t kr = kv_row(a.kv, max(pg[kt], 0), 0, t.g, kb + 16 * kt) + r;
             const unsigned char* kp = a.kv.codes + kr * (Q8 ? D : 2 * D) + gq * 16;
 #pragma unroll
-            for (int j = 0; j < KLD; ++j) kreg[kt][j] = *reinterpret_cast<const uint4*>(kp + 64 * j);
+            for (int j = 0; j < KLD; ++j) kreg[kt][j] = *reinterpret_cast<const u32x4_t*>(kp + 64 * j);
             if constexpr (Q8)
                 ksc[kt] = D == 128 ? *reinterpret_cast<const unsigned*>(a.kv.scales + kr * 4) : *reinterpret_cast<const u16*>(a.kv.scales + kr * 2);
         }
@@ -111,37 +112,51 @@ __global__ __launch_bounds__(256) void kv_attend_few_kernel(KvAttendArgs a) {
         for (int n = 0; n < NV; ++n) {
             const int k0 = n * RPI;  // the wave's first row of this load; all of them in one group of 16
             const size_t vr = kv_row(a.kv, max(pg[k0 >> 4], 0), 1, t.g, kb + k0) + lane / PPR;
-            vreg[n] = *reinterpret_cast<const uint4*>(a.kv.codes + vr * (Q8 ? D : 2 * D) + (lane % PPR) * 16);
+            vreg[n] = *reinterpret_cast<const u32x4_t*>(a.kv.codes + vr * (Q8 ? D : 2 * D) + (lane % PPR) * 16);
             if constexpr (Q8) vsc[n] = a.kv.scales[vr * (D / KV_BLOCK) + (lane % PPR) / 2];
         }
     };
 
-    int kb = t.s0 + wave * 32;
-    int pg[2] = {kv_page16(a, t, kb), kv_page16(a, t, kb + 16)};
-    if (kb < t.s1) load(kb, pg);
-    int pn[2] = {kv_page16(a, t, kb + 128), kv_page16(a, t, kb + 144)};
+    // this lane's page of a step ahead: lanes 0 and 1 (modulo 2) have those of the step's two groups of 16 keys
+    int kb = t.s0 + wave * 32, pv = -1;
+    int pg[2] = {-1, -1};
+    auto take = [&]() {
+        pg[0] = __builtin_amdgcn_readlane(pv, 0);
+        pg[1] = __builtin_amdgcn_readlane(pv, 1);
+    };
+    if (t.s0 < t.s1) {
+        pv = kv_page16(a, t, kb + 16 * (lane & 1));
+        take();
+        load(kb, pg);
+        pv = kv_page16(a, t, kb + 128 + 16 * (lane & 1));
+    }
     for (; kb < t.s1; kb += 128) {
         // V rows into this wave's image: rows outside the tile's range and holes as zeros
         const bool mixed = t.p0 != t.p1 && (kb + 31 > t.p0 || (a.window && kb <= t.p1 - a.window));
-        uint4 w[NV][Q8 ? 2 : 1];
+        const bool edge = mixed || kb < t.k_begin || kb + 32 > t.s1 || pg[0] < 0 || pg[1] < 0;
         bool bad = false;
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
-            const int key = kb + n * RPI + lane / PPR;
-            const bool in = key >= t.k_begin && key < t.s1 && pg[(n * RPI) >> 4] >= 0;
+            u32x4_t w[Q8 ? 2 : 1];
             if constexpr (Q8) {
                 const float f = kv_scale(vsc[n]);
-                w[n][0] = kv_decode8<FMT>(make_uint2(vreg[n].x, vreg[n].y), f);
-                w[n][1] = kv_decode8<FMT>(make_uint2(vreg[n].z, vreg[n].w), f);
+                w[0] = kv_decode8<FMT>(vreg[n].x, vreg[n].y, f);
+                w[1] = kv_decode8<FMT>(vreg[n].z, vreg[n].w, f);
             } else {
-                w[n][0] = vreg[n];
+                w[0] = vreg[n];
+            }
+            if (edge) {
+                const int key = kb + n * RPI + lane / PPR;
+                const bool in = key >= t.k_begin && key < t.s1 && pg[(n * RPI) >> 4] >= 0;
+#pragma unroll
+                for (int h = 0; h < (Q8 ? 2 : 1); ++h) {
+                    w[h] = keep(w[h], in);
+                    bad |= mixed && bf16x8_bad(w[h]);
+                }
             }
 #pragma unroll
-            for (int h = 0; h < (Q8 ? 2 : 1); ++h) {
-                if (!in) w[n][h] = make_uint4(0u, 0u, 0u, 0u);
-                if (mixed) bad |= bf16x8_bad(w[n][h]);
-                *reinterpret_cast<uint4*>(Vs + (n * RPI + lane / PPR) * LDV + (lane % PPR) * EPP + 8 * h) = w[n][h];
-            }
+            for (int h = 0; h < (Q8 ? 2 : 1); ++h)
+                *reinterpret_cast<u32x4_t*>(Vs + (n * RPI + lane / PPR) * LDV + (lane % PPR) * EPP + 8 * h) = w[h];
         }
         // scores of 2 x 16 keys: s[kt][i] = key kb + 16 kt + 4 gq + i
         f32x4_t s[2];
@@ -152,9 +167,9 @@ __global__ __launch_bounds__(256) void kv_attend_few_kernel(KvAttendArgs a) {
 #pragma unroll
                 for (int j = 0; j < KLD; ++j) {
                     const float f = kv_scale((ksc[kt] >> (8 * (2 * j + (gq >> 1)))) & 0xffu);
-                    const uint4 c = kreg[kt][j];
-                    s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kv_decode8<FMT>(make_uint2(c.x, c.y), f)), q[2 * j], s[kt], 0, 0, 0);
-                    s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kv_decode8<FMT>(make_uint2(c.z, c.w), f)), q[2 * j + 1], s[kt], 0, 0, 0);
+                    const u32x4_t c = kreg[kt][j];
+                    s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kv_decode8<FMT>(c.x, c.y, f)), q[2 * j], s[kt], 0, 0, 0);
+                    s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kv_decode8<FMT>(c.z, c.w, f)), q[2 * j + 1], s[kt], 0, 0, 0);
                 }
             } else {
 #pragma unroll
@@ -164,11 +179,9 @@ __global__ __launch_bounds__(256) void kv_attend_few_kernel(KvAttendArgs a) {
         }
         // the next rows travel while these go through the softmax
         const int pc[2] = {pg[0], pg[1]};
-        pg[0] = pn[0];
-        pg[1] = pn[1];
-        if (kb + 128 < t.s1) load(kb + 128, pg);
-        pn[0] = kv_page16(a, t, kb + 256);
-        pn[1] = kv_page16(a, t, kb + 272);
+        take();
+        load(kb + 128, pg);  // behind the part: page 0, not used
+        pv = kv_page16(a, t, kb + 256 + 16 * (lane & 1));
 
         float p[8], mx = -INFINITY;
 #pragma unroll
@@ -189,7 +202,7 @@ __global__ __launch_bounds__(256) void kv_attend_few_kernel(KvAttendArgs a) {
             ps += p[e];
         }
         l = l * alpha + ps;
-        const bf16x8_t ph = __builtin_bit_cast(bf16x8_t, make_uint4(pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]), pack_bf16(p[4], p[5]), pack_bf16(p[6], p[7])));
+        const bf16x8_t ph = __builtin_bit_cast(bf16x8_t, u32x4_t{pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]), pack_bf16(p[4], p[5]), pack_bf16(p[6], p[7])});
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) acc[dt] *= alpha;
         __builtin_amdgcn_wave_barrier();  // the image is this wave's own: its LDS accesses are served in order
@@ -207,8 +220,10 @@ __global__ __launch_bounds__(256) void kv_attend_few_kernel(KvAttendArgs a) {
 #pragma unroll
             for (int n = 0; n < NV; ++n)
 #pragma unroll
-                for (int h = 0; h < (Q8 ? 2 : 1); ++h)
-                    *reinterpret_cast<uint4*>(Vs + (n * RPI + lane / PPR) * LDV + (lane % PPR) * EPP + 8 * h) = bf16x8_clean(w[n][h]);
+                for (int h = 0; h < (Q8 ? 2 : 1); ++h) {
+                    u32x4_t* p = reinterpret_cast<u32x4_t*>(Vs + (n * RPI + lane / PPR) * LDV + (lane % PPR) * EPP + 8 * h);
+                    *p = bf16x8_clean(*p);
+                }
             __builtin_amdgcn_wave_barrier();
         }
         const u16* vrow = Vs + (4 * gq + (r >> 2)) * LDV + 4 * (r & 3);
@@ -316,7 +331,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
     float m = -INFINITY, l = 0.f;
     const float sc = a.scale * 1.4426950408889634f;
 
-    uint4 kreg[NP], vreg[NP];
+    u32x4_t kreg[NP], vreg[NP];
     unsigned ksc[NP], vsc[NP];
     const int krow = lane / PPR, pc = lane % PPR;
     auto load = [&](int kb, const int (&pg)[4]) {
@@ -325,57 +340,63 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
             const int k0 = (n * 4 + wave) * KPW;  // the wave's first key of this pass; all of them in one group of 16
             const size_t kr = kv_row(a.kv, max(pg[k0 >> 4], 0), 0, t.g, kb + k0) + krow;
             const size_t vr = kr + ((size_t)a.kv.nkv << a.kv.page_shift);
-            kreg[n] = *reinterpret_cast<const uint4*>(a.kv.codes + kr * (Q8 ? D : 2 * D) + pc * 16);
-            vreg[n] = *reinterpret_cast<const uint4*>(a.kv.codes + vr * (Q8 ? D : 2 * D) + pc * 16);
+            kreg[n] = *reinterpret_cast<const u32x4_t*>(a.kv.codes + kr * (Q8 ? D : 2 * D) + pc * 16);
+            vreg[n] = *reinterpret_cast<const u32x4_t*>(a.kv.codes + vr * (Q8 ? D : 2 * D) + pc * 16);
             if constexpr (Q8) {
                 ksc[n] = a.kv.scales[kr * (D / KV_BLOCK) + pc / 2];
                 vsc[n] = a.kv.scales[vr * (D / KV_BLOCK) + pc / 2];
             }
         }
     };
-    auto pages = [&](int kb, int (&pg)[4]) {
+    // lanes 0 .. 3 (modulo 4) have the pages of the next block's four groups of 16 keys
+    int pv = -1, pg[4] = {-1, -1, -1, -1};
+    auto take = [&]() {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pg[i] = kv_page16(a, t, kb + 16 * i);
+        for (int i = 0; i < 4; ++i) pg[i] = __builtin_amdgcn_readlane(pv, i);
     };
-
-    int pg[4], pn[4];
-    pages(t.s0, pg);
-    if (t.s0 < t.s1) load(t.s0, pg);
-    pages(t.s0 + KB, pn);
+    if (t.s0 < t.s1) {
+        pv = kv_page16(a, t, t.s0 + 16 * (lane & 3));
+        take();
+        load(t.s0, pg);
+        pv = kv_page16(a, t, t.s0 + KB + 16 * (lane & 3));
+    }
     if (threadIdx.x == 0) sh_bad = -1;
     for (int kb = t.s0; kb < t.s1; kb += KB) {
         const bool mixed = kb + KB - 1 > t.p0 || (a.window && kb <= t.p1 - a.window);
-        uint4 w[NP][Q8 ? 2 : 1];
+        const bool edge = mixed || kb < t.k_begin || kb + KB > t.s1 || (pg[0] | pg[1] | pg[2] | pg[3]) < 0;
         __syncthreads();  // every wave is done with the previous image
         bool bad = false;
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
             const int k0 = (n * 4 + wave) * KPW;
             const int key = k0 + krow;
-            const bool in = kb + key >= t.k_begin && kb + key < t.s1 && pg[k0 >> 4] >= 0;
+            u32x4_t w[Q8 ? 2 : 1];
             if constexpr (Q8) {
                 const float fk = kv_scale(ksc[n]), fv = kv_scale(vsc[n]);
-                *reinterpret_cast<uint4*>(Ks + key * LDK + pc * 16) = kv_decode8<FMT>(make_uint2(kreg[n].x, kreg[n].y), fk);
-                *reinterpret_cast<uint4*>(Ks + key * LDK + pc * 16 + 8) = kv_decode8<FMT>(make_uint2(kreg[n].z, kreg[n].w), fk);
-                w[n][0] = kv_decode8<FMT>(make_uint2(vreg[n].x, vreg[n].y), fv);
-                w[n][1] = kv_decode8<FMT>(make_uint2(vreg[n].z, vreg[n].w), fv);
+                *reinterpret_cast<u32x4_t*>(Ks + key * LDK + pc * 16) = kv_decode8<FMT>(kreg[n].x, kreg[n].y, fk);
+                *reinterpret_cast<u32x4_t*>(Ks + key * LDK + pc * 16 + 8) = kv_decode8<FMT>(kreg[n].z, kreg[n].w, fk);
+                w[0] = kv_decode8<FMT>(vreg[n].x, vreg[n].y, fv);
+                w[1] = kv_decode8<FMT>(vreg[n].z, vreg[n].w, fv);
             } else {
-                *reinterpret_cast<uint4*>(Ks + key * LDK + pc * 8) = kreg[n];
-                w[n][0] = vreg[n];
+                *reinterpret_cast<u32x4_t*>(Ks + key * LDK + pc * 8) = kreg[n];
+                w[0] = vreg[n];
+            }
+            if (edge) {
+                const bool in = kb + key >= t.k_begin && kb + key < t.s1 && pg[k0 >> 4] >= 0;
+#pragma unroll
+                for (int h = 0; h < (Q8 ? 2 : 1); ++h) {
+                    w[h] = keep(w[h], in);
+                    bad |= mixed && bf16x8_bad(w[h]);
+                }
             }
 #pragma unroll
-            for (int h = 0; h < (Q8 ? 2 : 1); ++h) {
-                if (!in) w[n][h] = make_uint4(0u, 0u, 0u, 0u);
-                if (mixed) bad |= bf16x8_bad(w[n][h]);
-                *reinterpret_cast<uint4*>(Vs + key * LDV + pc * EPP + 8 * h) = w[n][h];
-            }
+            for (int h = 0; h < (Q8 ? 2 : 1); ++h) *reinterpret_cast<u32x4_t*>(Vs + key * LDV + pc * EPP + 8 * h) = w[h];
         }
         if (bad) sh_bad = kb;
-        int pcur[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { pcur[i] = pg[i]; pg[i] = pn[i]; }
-        if (kb + KB < t.s1) load(kb + KB, pg);
-        pages(kb + 2 * KB, pn);
+        const int pcur[4] = {pg[0], pg[1], pg[2], pg[3]};
+        take();
+        load(kb + KB, pg);  // behind the part: page 0, not used
+        pv = kv_page16(a, t, kb + 2 * KB + 16 * (lane & 3));
         __syncthreads();
         if (mixed && sh_bad == kb) {
             if (wlive) {
@@ -393,8 +414,10 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
 #pragma unroll
             for (int n = 0; n < NP; ++n)
 #pragma unroll
-                for (int h = 0; h < (Q8 ? 2 : 1); ++h)
-                    *reinterpret_cast<uint4*>(Vs + ((n * 4 + wave) * KPW + krow) * LDV + pc * EPP + 8 * h) = bf16x8_clean(w[n][h]);
+                for (int h = 0; h < (Q8 ? 2 : 1); ++h) {
+                    u32x4_t* p = reinterpret_cast<u32x4_t*>(Vs + ((n * 4 + wave) * KPW + krow) * LDV + pc * EPP + 8 * h);
+                    *p = bf16x8_clean(*p);
+                }
             __syncthreads();
         }
         // wave-uniform: no row of this wave sees the block
@@ -411,7 +434,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
                 s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8_t*>(kp + 16 * j), q[j], s[kt], 0, 0, 0);
         }
         // s[kt][i] = key kb + 32 kt + 8 (i / 4) + 4 hf + i % 4 of this lane's row
-        const bool whole = kb + KB - 1 <= wp0 && !(a.window && kb <= wp1 - a.window) && kb + KB <= t.s1 && pcur[0] >= 0 && pcur[1] >= 0 && pcur[2] >= 0 && pcur[3] >= 0;
+        const bool whole = kb + KB - 1 <= wp0 && !(a.window && kb <= wp1 - a.window) && kb + KB <= t.s1 && (pcur[0] | pcur[1] | pcur[2] | pcur[3]) >= 0;
         if (!whole) {
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
@@ -447,7 +470,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
                     p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][8 * u + e], sc, -ref));
                     l += p[e];
                 }
-                const bf16x8_t ph = __builtin_bit_cast(bf16x8_t, make_uint4(pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]), pack_bf16(p[4], p[5]), pack_bf16(p[6], p[7])));
+                const bf16x8_t ph = __builtin_bit_cast(bf16x8_t, u32x4_t{pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]), pack_bf16(p[4], p[5]), pack_bf16(p[6], p[7])});
                 const u16* vrow = Vs + (32 * kt + 16 * u + 4 * hf + ((lane & 15) >> 2)) * LDV + (lane & 16) + 4 * (lane & 3);
 #pragma unroll
                 for (int dt = 0; dt < NDT; ++dt)

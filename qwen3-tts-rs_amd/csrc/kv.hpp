@@ -25,7 +25,7 @@ struct KvLayer {
     int format, nkv, d;
     int page_shift;         // log2 of the tokens per page: at least 4, so that 16 keys that start at a multiple of 16 share a page
     int n_pages, max_pages;
-    const int* page_table;  // [row][max_pages], entries outside [0, n_pages) are holes; null: row r owns pages r max_pages ..
+    const int* page_table;  // [row][max_pages], entries outside [0, n_pages) are holes
 };
 
 // The sequences of a call.  Sequence b's new tokens are rows q_start[b] .. q_start[b + 1] - 1 of the call's tensors and, the last
@@ -79,8 +79,7 @@ struct KvAttendPlan {
 void launch_kv_attend(hipStream_t st, KvAttendArgs a, const KvAttendPlan& p);
 
 // one launch with its error as an exception (hipGetLastError would also report what other code left there)
-// The talker's cache in 8 bits (generate.cpp): rows that own consecutive pages, as KVView without a table, and the batch of the
-// launch at hand.  The plan does not depend on what else is in the batch: single tokens in parts of KV_TALKER_PART keys, prompts in
+// The talker's cache in 8 bits (generate.cpp): rows that own consecutive pages, and the batch of the launch at hand.  The plan does not depend on what else is in the batch: single tokens in parts of KV_TALKER_PART keys, prompts in
 // tiles with all of their keys, so that a row's result is the same whatever rows it shares a launch with.
 constexpr int KV_TALKER_PART = 512;
 struct KvStack {

@@ -5,6 +5,8 @@
 
 namespace qtts {
 
+typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));  // register arrays of HIP's uint4 end in scratch memory
+
 // biased exponent of a block's scale from the largest |x| (as bits): see KvFormat.  448 = 1.75 2^8 and 127 = 1.984375 2^6.
 template <int FMT>
 __device__ __forceinline__ int kv_scale_exp(unsigned amax_bits) {
@@ -53,11 +55,11 @@ __device__ __forceinline__ unsigned pack_bf16(float a, float b) {
 }
 // eight codes -> eight bf16 in operand order, exact (see KvFormat)
 template <int FMT>
-__device__ __forceinline__ uint4 kv_decode8(uint2 c, float scale) {
+__device__ __forceinline__ u32x4_t kv_decode8(unsigned c0, unsigned c1, float scale) {
     float f[8];
-    kv_decode4<FMT>(c.x, scale, f);
-    kv_decode4<FMT>(c.y, scale, f + 4);
-    return make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+    kv_decode4<FMT>(c0, scale, f);
+    kv_decode4<FMT>(c1, scale, f + 4);
+    return u32x4_t{pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7])};
 }
 
 }  // namespace qtts

@@ -33,9 +33,7 @@ QTTS_KV_HD KvSeq kv_seq(const KvBatch& b, int s) {
 }
 // physical page of a position, -1 = hole
 QTTS_KV_HD int kv_page(const KvLayer& kv, int row, int pos) {
-    const long i = (long)row * kv.max_pages + (pos >> kv.page_shift);
-    if (!kv.page_table) return (int)i;
-    const int p = kv.page_table[i];
+    const int p = kv.page_table[(long)row * kv.max_pages + (pos >> kv.page_shift)];
     return (unsigned)p < (unsigned)kv.n_pages ? p : -1;
 }
 // index of a head row within the layer (its elements start at index * d, its scales at index * d / 32)
@@ -76,9 +74,12 @@ QTTS_KV_HD KvTile kv_tile(const KvAttendArgs& a, int pair, int tile, int part) {
     t.live = part < t.parts;
     return t;
 }
-// page of the 16 keys from `key` on, -1 = hole or past the part; key is a multiple of 16 and the same in every lane
+// page of the keys from `key`, a multiple of 16, up to the next one, -1 = hole or past the part.  Only for parts with keys.  The kernels
+// load it a step ahead, one lane per group of 16 keys, and hand it out with a lane read: as an ordinary scalar of the loop it is a
+// load and a wait for everything in flight.
 QTTS_KV_HD int kv_page16(const KvAttendArgs& a, const KvTile& t, int key) {
-    return key < t.s1 ? kv_page(a.kv, t.s.row, key) : -1;
+    const int p = kv_page(a.kv, t.s.row, kv_min(key, t.s1 - 1));
+    return key < t.s1 ? p : -1;
 }
 
 // ---- host

@@ -34,7 +34,7 @@ static int tiles(const KvAttendArgs& a, int trial) {
                     const size_t r = kv_row(a.kv, p < 0 ? 0 : p, 1, t.g, key) + 15;
                     NEED(r < ((size_t)a.kv.n_pages * 2 * a.kv.nkv << a.kv.page_shift));
                 }
-                NEED(kv_page16(a, t, (t.s1 + 15) & ~15) == -1);
+                if (t.s0 < t.s1) NEED(kv_page16(a, t, (t.s1 + 15) & ~15) == -1);
             }
     return 0;
 }
