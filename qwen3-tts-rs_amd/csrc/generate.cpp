@@ -345,9 +345,11 @@ static void generate_impl(Model& m, const qtts_request* reqs, int n, const qtts_
             kv8.base.page_table = g.kv8_pages.as<int>();
             kv8.layer_rows = head_rows;
             // decode steps: token b is row b's newest
-            const int tiles = (c.talker.nh / c.talker.nkv + 15) / 16, parts = (max_pages * PAGE_TOKENS + KV_TALKER_PART - 1) / KV_TALKER_PART;
+            int part = KV_TALKER_PART;
+            while ((max_pages * PAGE_TOKENS + part - 1) / part > KV_MAX_PARTS) part *= 2;
+            const int tiles = (c.talker.nh / c.talker.nkv + 15) / 16, parts = (max_pages * PAGE_TOKENS + part - 1) / part;
             kv8.batch = KvBatch{B, B, 1, max_pages * PAGE_TOKENS, nullptr, reinterpret_cast<const int*>(g.toks_dec.as<Tok>()) + 1, (int)(sizeof(Tok) / sizeof(int)), 1, nullptr};
-            kv8.plan = KvAttendPlan{16, tiles, parts, KV_TALKER_PART, (size_t)B * c.talker.nkv * tiles * parts * 16 * (c.talker.d + 2) * sizeof(float)};
+            kv8.plan = KvAttendPlan{16, tiles, parts, part, (size_t)B * c.talker.nkv * tiles * parts * 16 * (c.talker.d + 2) * sizeof(float)};
             if (parts > 1) g.kv8_ws.ensure(kv8.plan.ws_bytes);
             kv8.ws = g.kv8_ws.as<float>();
         }

@@ -1,103 +1,131 @@
 // Writing keys and values into the paged cache and reading them back (gfx950), and the talker's projection pass that ends in it.
 //
-// A thread owns 16 consecutive elements of a head row, so that 8-bit codes leave and enter in 16-byte accesses; two neighbouring
-// lanes hold a block of 32 and share its largest element with one lane swap.  Nothing is reused: both kernels are bound by the
-// bytes they move.
+// Both directions are bound by the bytes they move; nothing is reused.  A lane owns 16 bytes of a row of the caller's tensor, so that
+// one access of a wave is contiguous there (64-byte pieces per lane cost the f32 read back half its rate: 26 us instead of 18 us for
+// 84 MB), 8 or 4 codes of the cache, and a quarter or an eighth of a block of 32 whose largest element goes round by lane swaps.  A
+// block of threads stays with one head while there are many tokens, so that its rows are neighbours in the cache's pages, and with
+// one token otherwise; a thread has four rows in flight.
 #include "kv_device.hpp"
 
 #include <algorithm>
 
 namespace qtts {
 
-__device__ __forceinline__ void load16(const float* p, float (&x)[16]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(x + 4 * i) = *reinterpret_cast<const float4*>(p + 4 * i);
+constexpr int KV_MOVE_UNROLL = 4;
+
+template <int CTRL>
+__device__ __forceinline__ unsigned dpp_max(unsigned v) {
+    return max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false));
 }
-__device__ __forceinline__ void load16(const bf16_t* p, float (&x)[16]) {
-    float a[8], b[8];
-    load8(p, a);
-    load8(p + 8, b);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) { x[i] = a[i]; x[8 + i] = b[i]; }
+// largest value of the 4 or 8 neighbouring lanes that hold a block, left in all of them
+template <int LANES>
+__device__ __forceinline__ unsigned block_max(unsigned v) {
+    v = dpp_max<0xb1>(v);                          // quad_perm 1 0 3 2
+    v = dpp_max<0x4e>(v);                          // quad_perm 2 3 0 1
+    if constexpr (LANES == 8) v = dpp_max<0x141>(v);  // row_half_mirror
+    return v;
 }
-template <typename T>
-__device__ __forceinline__ void store16(T* p, const float (&x)[16]) {
-    float a[8], b[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) { a[i] = x[i]; b[i] = x[8 + i]; }
-    store8(p, a);
-    store8(p + 8, b);
+__device__ __forceinline__ void load_piece(const bf16_t* p, float (&x)[8]) { load8(p, x); }
+__device__ __forceinline__ void load_piece(const float* p, float (&x)[4]) {
+    const float4 v = *reinterpret_cast<const float4*>(p);
+    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+}
+__device__ __forceinline__ void load_piece(const bf16_t* p, float (&x)[4]) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xffff0000u);
+    x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xffff0000u);
+}
+__device__ __forceinline__ void store_piece(bf16_t* p, const float (&x)[8]) {
+    *reinterpret_cast<u32x4_t*>(p) = u32x4_t{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
+}
+__device__ __forceinline__ void store_piece(float* p, const float (&x)[4]) { *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]); }
+__device__ __forceinline__ void store_piece(bf16_t* p, const float (&x)[4]) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
 }
 
-// grid: x = sequence, y = pieces of the sequence's rows (strided), z = keys | values
+// grid: x = sequence, y = tokens, z = (keys | values) x heads; a.head_shift: log2 of the heads a block covers
 template <typename T, int FMT, int D, bool WRITE>
 __global__ __launch_bounds__(256) void kv_move_kernel(KvMoveArgs a) {
-    constexpr int LPR = D / 16, RPB = 256 / LPR;  // lanes per row, rows per block
+    constexpr int EPT = 16 / (int)sizeof(T), LPR = D / EPT, RPB = 256 / LPR, U = KV_MOVE_UNROLL;  // elements a lane owns, lanes per row, rows per pass
     const KvSeq s = kv_seq(a.b, blockIdx.x);
-    const int which = blockIdx.z, sub = threadIdx.x % LPR;
+    const int zh = (int)gridDim.z >> 1, which = (int)blockIdx.z >= zh, sub = threadIdx.x % LPR;
+    const int rib = threadIdx.x / LPR, g = (((int)blockIdx.z - (which ? zh : 0)) << a.head_shift) + (rib & ((1 << a.head_shift) - 1));
+    const int tpp = RPB >> a.head_shift;  // tokens per pass
+    if (g >= a.kv.nkv) return;            // uniform over a row's lanes
     const long ts = which ? a.v_token_stride : a.k_token_stride, hs = which ? a.v_head_stride : a.k_head_stride;
-    const T* src = (const T*)(which ? a.v_in : a.k_in);
-    T* dst = (T*)(which ? a.v_out : a.k_out);
-    const int nkv = a.kv.nkv;
-    const long rows = (long)s.n * nkv;
-    for (long r = (long)blockIdx.y * RPB + threadIdx.x / LPR; r < rows; r += (long)gridDim.y * RPB) {
-        const int i = (int)(r / nkv), g = (int)(r - (long)i * nkv);
-        const int pos = s.ctx - s.n + i;
-        const int page = pos >= 0 ? kv_page(a.kv, s.row, pos) : -1;
-        const long off = (long)(s.t0 + i) * ts + (long)g * hs + sub * 16;
-        if constexpr (WRITE) {
-            if (page < 0) continue;  // uniform over the row's lanes
-            const size_t row = kv_row(a.kv, page, which, g, pos);
-            float x[16];
-            load16(src + off, x);
-            if constexpr (FMT == KV_BF16) {
-                store16((bf16_t*)a.kv.codes + row * D + sub * 16, x);
-            } else {
-                unsigned m = 0;
+    const T* src = (const T*)(which ? a.v_in : a.k_in) + (long)g * hs + sub * EPT;
+    T* dst = (T*)(which ? a.v_out : a.k_out) + (long)g * hs + sub * EPT;
+    for (int i0 = (int)blockIdx.y * tpp * U + (rib >> a.head_shift); i0 < s.n; i0 += (int)gridDim.y * tpp * U) {
+        int page[U];
+        float x[U][EPT];
+        size_t row[U];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) m = max(m, __float_as_uint(x[e]) & 0x7fffffffu);
-                m = max(m, (unsigned)__shfl_xor((int)m, 1, 64));
-                const bool bad = m >= 0x7f800000u;
-                const int ex = bad ? kv_bad_exp<FMT>() : kv_scale_exp<FMT>(m);
-                const float inv = __uint_as_float((unsigned)(254 - (bad ? 127 : ex)) << 23);
-                uint4 c;
-                c.x = kv_encode4<FMT>(x, inv);
-                c.y = kv_encode4<FMT>(x + 4, inv);
-                c.z = kv_encode4<FMT>(x + 8, inv);
-                c.w = kv_encode4<FMT>(x + 12, inv);
-                if (bad) c.x = c.y = c.z = c.w = kv_bad_codes<FMT>();
-                *reinterpret_cast<uint4*>(a.kv.codes + row * D + sub * 16) = c;
-                if ((sub & 1) == 0) a.kv.scales[row * (D / KV_BLOCK) + (sub >> 1)] = (unsigned char)ex;
-            }
-        } else {
-            float x[16];
-            if (page < 0) {
+        for (int k = 0; k < U; ++k) {
+            const int i = i0 + k * tpp, pos = s.ctx - s.n + i;
+            page[k] = i < s.n && pos >= 0 ? kv_page(a.kv, s.row, pos) : -1;
+            if constexpr (WRITE) load_piece(src + (long)(s.t0 + min(i, s.n - 1)) * ts, x[k]);
+        }
+        if constexpr (!WRITE) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = 0.f;
-            } else {
-                const size_t row = kv_row(a.kv, page, which, g, pos);
+            for (int k = 0; k < U; ++k) {
+                // holes and rows past the end read page 0, which is there, and drop it
+                row[k] = kv_row(a.kv, max(page[k], 0), which, g, s.ctx - s.n + i0 + k * tpp);
                 if constexpr (FMT == KV_BF16) {
-                    load16((const bf16_t*)a.kv.codes + row * D + sub * 16, x);
+                    load_piece((const bf16_t*)a.kv.codes + row[k] * D + sub * EPT, x[k]);
                 } else {
-                    const uint4 c = *reinterpret_cast<const uint4*>(a.kv.codes + row * D + sub * 16);
-                    const float sc = kv_scale(a.kv.scales[row * (D / KV_BLOCK) + (sub >> 1)]);
-                    kv_decode4<FMT>(c.x, sc, x);
-                    kv_decode4<FMT>(c.y, sc, x + 4);
-                    kv_decode4<FMT>(c.z, sc, x + 8);
-                    kv_decode4<FMT>(c.w, sc, x + 12);
+                    const unsigned char* cp = a.kv.codes + row[k] * D + sub * EPT;
+                    const float sc = kv_scale(a.kv.scales[row[k] * (D / KV_BLOCK) + sub * EPT / KV_BLOCK]);
+                    if constexpr (EPT == 8) {
+                        const uint2 c = *reinterpret_cast<const uint2*>(cp);
+                        kv_decode4<FMT>(c.x, sc, x[k]);
+                        kv_decode4<FMT>(c.y, sc, x[k] + 4);
+                    } else {
+                        kv_decode4<FMT>(*reinterpret_cast<const unsigned*>(cp), sc, x[k]);
+                    }
                 }
             }
-            store16(dst + off, x);
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const int i = i0 + k * tpp;
+            if constexpr (WRITE) {
+                unsigned m = 0;
+#pragma unroll
+                for (int e = 0; e < EPT; ++e) m = max(m, __float_as_uint(x[k][e]) & 0x7fffffffu);
+                if constexpr (FMT != KV_BF16) m = block_max<KV_BLOCK / EPT>(m);
+                if (page[k] < 0) continue;
+                row[k] = kv_row(a.kv, page[k], which, g, s.ctx - s.n + i);
+                if constexpr (FMT == KV_BF16) {
+                    store_piece((bf16_t*)a.kv.codes + row[k] * D + sub * EPT, x[k]);
+                } else {
+                    const bool bad = m >= 0x7f800000u;
+                    const int ex = bad ? kv_bad_exp<FMT>() : kv_scale_exp<FMT>(m);
+                    const float inv = __uint_as_float((unsigned)(254 - (bad ? 127 : ex)) << 23);
+                    unsigned char* cp = a.kv.codes + row[k] * D + sub * EPT;
+                    const unsigned c0 = bad ? kv_bad_codes<FMT>() : kv_encode4<FMT>(x[k], inv);
+                    if constexpr (EPT == 8) *reinterpret_cast<uint2*>(cp) = make_uint2(c0, bad ? kv_bad_codes<FMT>() : kv_encode4<FMT>(x[k] + 4, inv));
+                    else *reinterpret_cast<unsigned*>(cp) = c0;
+                    if (sub % (KV_BLOCK / EPT) == 0) a.kv.scales[row[k] * (D / KV_BLOCK) + sub * EPT / KV_BLOCK] = (unsigned char)ex;
+                }
+            } else if (i < s.n) {
+                if (page[k] < 0) {
+#pragma unroll
+                    for (int e = 0; e < EPT; ++e) x[k][e] = 0.f;
+                }
+                store_piece(dst + (long)(s.t0 + i) * ts, x[k]);
+            }
         }
     }
 }
 
 template <bool WRITE>
-static void launch_kv_move(hipStream_t st, int dtype, const KvMoveArgs& a) {
-    if (a.b.n_seq == 0 || a.b.n_tokens == 0) return;
-    const int rpb = 256 / (a.kv.d / 16);
-    const long pieces = ((long)a.b.max_new * a.kv.nkv + rpb - 1) / rpb;
-    const dim3 grid((unsigned)a.b.n_seq, (unsigned)std::min<long>(pieces, 65535), 2);
+static void launch_kv_move(hipStream_t st, int dtype, KvMoveArgs a) {
+    if (a.b.n_seq == 0 || a.b.n_tokens == 0 || a.b.max_new == 0) return;
+    const int rpb = 256 / (a.kv.d * (int)dtype_size(dtype) / 16);  // rows per pass
+    a.head_shift = 0;
+    while ((2 << a.head_shift) <= rpb && (1 << a.head_shift) < a.kv.nkv) ++a.head_shift;
+    const long tokens = (long)(rpb >> a.head_shift) * KV_MOVE_UNROLL, heads = (a.kv.nkv + (1 << a.head_shift) - 1) >> a.head_shift;
+    const dim3 grid((unsigned)a.b.n_seq, (unsigned)std::min<long>((a.b.max_new + tokens - 1) / tokens, 65535), (unsigned)(2 * heads));
 #define QTTS_KV_MOVE(T, FMT, DD) \
     if (a.kv.format == FMT && a.kv.d == DD) return kv_launch(kv_move_kernel<T, FMT, DD, WRITE>, grid, dim3(256), st, a);
 #define QTTS_KV_MOVE_T(T)           \

@@ -54,7 +54,7 @@ __device__ __forceinline__ float bad_only(u16 b) { return (b & 0x7f80u) == 0x7f8
 
 // ---------------------------------------------------------------------------------------------- at most 16 rows a tile
 template <int FMT, int D>
-__global__ __launch_bounds__(256) void kv_attend_few_kernel(KvAttendArgs a) {
+__global__ __launch_bounds__(256, 3) void kv_attend_few_kernel(KvAttendArgs a) {
     constexpr bool Q8 = FMT != KV_BF16;
     constexpr int NJ = D / 32, NDT = D / 16;
     constexpr int KLD = Q8 ? D / 64 : D / 32;          // 16-byte loads of a K row per lane
@@ -98,22 +98,28 @@ __global__ __launch_bounds__(256) void kv_attend_few_kernel(KvAttendArgs a) {
 
     u32x4_t kreg[2][KLD], vreg[NV];
     unsigned ksc[2], vsc[NV];
+    // a page is the same for all lanes: scalar base, constant lane offsets
+    constexpr unsigned ROWB = Q8 ? D : 2 * D;  // bytes of a head row
+    const unsigned koff = r * ROWB + gq * 16, voff = (lane / PPR) * ROWB + (lane % PPR) * 16, vsoff = (lane / PPR) * (D / KV_BLOCK) + (lane % PPR) / 2;
     auto load = [&](int kb, const int (&pg)[2]) {
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
-            const size_t kr = kv_row(a.kv, max(pg[kt], 0), 0, t.g, kb + 16 * kt) + r;
-            const unsigned char* kp = a.kv.codes + kr * (Q8 ? D : 2 * D) + gq * 16;
+            // a hole is read as page 0: in bounds, and what it holds is masked
+            const size_t kr = kv_row(a.kv, max(pg[kt], 0), 0, t.g, kb + 16 * kt);
+            const unsigned char* kp = a.kv.codes + kr * ROWB;
 #pragma unroll
-            for (int j = 0; j < KLD; ++j) kreg[kt][j] = *reinterpret_cast<const u32x4_t*>(kp + 64 * j);
-            if constexpr (Q8)
-                ksc[kt] = D == 128 ? *reinterpret_cast<const unsigned*>(a.kv.scales + kr * 4) : *reinterpret_cast<const u16*>(a.kv.scales + kr * 2);
+            for (int j = 0; j < KLD; ++j) kreg[kt][j] = *reinterpret_cast<const u32x4_t*>(kp + (koff + 64 * j));
+            if constexpr (Q8) {
+                const unsigned char* sp = a.kv.scales + kr * (D / KV_BLOCK);
+                ksc[kt] = D == 128 ? *reinterpret_cast<const unsigned*>(sp + (unsigned)r * 4) : *reinterpret_cast<const u16*>(sp + (unsigned)r * 2);
+            }
         }
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
             const int k0 = n * RPI;  // the wave's first row of this load; all of them in one group of 16
-            const size_t vr = kv_row(a.kv, max(pg[k0 >> 4], 0), 1, t.g, kb + k0) + lane / PPR;
-            vreg[n] = *reinterpret_cast<const u32x4_t*>(a.kv.codes + vr * (Q8 ? D : 2 * D) + (lane % PPR) * 16);
-            if constexpr (Q8) vsc[n] = a.kv.scales[vr * (D / KV_BLOCK) + (lane % PPR) / 2];
+            const size_t vr = kv_row(a.kv, max(pg[k0 >> 4], 0), 1, t.g, kb + k0);
+            vreg[n] = *reinterpret_cast<const u32x4_t*>(a.kv.codes + vr * ROWB + voff);
+            if constexpr (Q8) vsc[n] = (a.kv.scales + vr * (D / KV_BLOCK))[vsoff];
         }
     };
 
@@ -334,17 +340,18 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
     u32x4_t kreg[NP], vreg[NP];
     unsigned ksc[NP], vsc[NP];
     const int krow = lane / PPR, pc = lane % PPR;
+    constexpr unsigned ROWB = Q8 ? D : 2 * D;  // bytes of a head row
+    const unsigned loff = krow * ROWB + pc * 16, lsoff = krow * (D / KV_BLOCK) + pc / 2;
     auto load = [&](int kb, const int (&pg)[4]) {
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
             const int k0 = (n * 4 + wave) * KPW;  // the wave's first key of this pass; all of them in one group of 16
-            const size_t kr = kv_row(a.kv, max(pg[k0 >> 4], 0), 0, t.g, kb + k0) + krow;
-            const size_t vr = kr + ((size_t)a.kv.nkv << a.kv.page_shift);
-            kreg[n] = *reinterpret_cast<const u32x4_t*>(a.kv.codes + kr * (Q8 ? D : 2 * D) + pc * 16);
-            vreg[n] = *reinterpret_cast<const u32x4_t*>(a.kv.codes + vr * (Q8 ? D : 2 * D) + pc * 16);
+            const size_t kr = kv_row(a.kv, max(pg[k0 >> 4], 0), 0, t.g, kb + k0), vr = kr + ((size_t)a.kv.nkv << a.kv.page_shift);
+            kreg[n] = *reinterpret_cast<const u32x4_t*>(a.kv.codes + kr * ROWB + loff);
+            vreg[n] = *reinterpret_cast<const u32x4_t*>(a.kv.codes + vr * ROWB + loff);
             if constexpr (Q8) {
-                ksc[n] = a.kv.scales[kr * (D / KV_BLOCK) + pc / 2];
-                vsc[n] = a.kv.scales[vr * (D / KV_BLOCK) + pc / 2];
+                ksc[n] = (a.kv.scales + kr * (D / KV_BLOCK))[lsoff];
+                vsc[n] = (a.kv.scales + vr * (D / KV_BLOCK))[lsoff];
             }
         }
     };
@@ -506,43 +513,52 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
 }
 
 // ------------------------------------------------------------------------------------------------ joining the parts
+// One wave per row: its lanes take the parts' maxima and sums (64 at a time) and turn them into weights; then each lane adds up its
+// D / 64 columns of the parts' outputs with eight loads in flight.
 template <int TR, int D>
 __global__ __launch_bounds__(256) void kv_attend_join_kernel(KvAttendArgs a) {
-    constexpr int EPT = D / 16;
+    constexpr int EPL = D / 64;
+    typedef float vec_t __attribute__((ext_vector_type(EPL)));
     const int unit = blockIdx.x, pair = unit / a.tiles, tile = unit - pair * a.tiles;
     const KvTile t = kv_tile<TR>(a, pair, tile, 0);
-    const int orow = blockIdx.y * 16 + (threadIdx.x >> 4), d0 = (threadIdx.x & 15) * EPT;
-    const int rr = t.row0 + orow;
+    const int lane = threadIdx.x & 63, trow = (int)blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rr = t.row0 + trow;
     if (!t.live || t.parts == 1 || rr >= t.rows) return;
-    const size_t u = (size_t)unit * a.splits * TR + orow;
+    const size_t u = (size_t)unit * a.splits * TR + trow;
     const float* ml = a.ws + (size_t)a.b.n_seq * a.kv.nkv * a.tiles * a.splits * TR * D + u * 2;
-    const float* po = a.ws + u * D + d0;
+    const float* po = a.ws + u * D + lane * EPL;
     float M = -INFINITY;
-    for (int s = 0; s < t.parts; ++s) M = fmaxf(M, ml[(size_t)s * TR * 2]);
+    for (int s = lane; s < t.parts; s += 64) M = fmaxf(M, ml[(size_t)s * TR * 2]);
+    M = wave_max(M);
     const float ref = M == -INFINITY ? 0.f : M;
-    float L = 0.f, o[EPT];
+    float L = 0.f;
+    vec_t o;
 #pragma unroll
-    for (int e = 0; e < EPT; ++e) o[e] = 0.f;
-    for (int s = 0; s < t.parts; ++s) {
-        const float wt = __builtin_amdgcn_exp2f(ml[(size_t)s * TR * 2] - ref);
-        L += wt * ml[(size_t)s * TR * 2 + 1];
+    for (int e = 0; e < EPL; ++e) o[e] = 0.f;
+    for (int s0 = 0; s0 < t.parts; s0 += 64) {
+        const int n = min(t.parts - s0, 64);
+        float w = 0.f;  // weight of part s0 + lane
+        if (lane < n) {
+            w = __builtin_amdgcn_exp2f(ml[(size_t)(s0 + lane) * TR * 2] - ref);
+            L += w * ml[(size_t)(s0 + lane) * TR * 2 + 1];
+        }
+        for (int s = 0; s < n; s += 8) {
+            vec_t v[8];
 #pragma unroll
-        for (int e = 0; e < EPT; e += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(po + (size_t)s * TR * D + e);
-            o[e] += wt * v.x;
-            o[e + 1] += wt * v.y;
-            o[e + 2] += wt * v.z;
-            o[e + 3] += wt * v.w;
+            for (int k = 0; k < 8; ++k) v[k] = *reinterpret_cast<const vec_t*>(po + (size_t)(s0 + min(s + k, n - 1)) * TR * D);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float wk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), min(s + k, n - 1)));
+#pragma unroll
+                for (int e = 0; e < EPL; ++e) o[e] += s + k < n ? wk * v[k][e] : 0.f;
+            }
         }
     }
+    L = wave_sum(L);
     const int tk = rr / t.G, hd = t.g * t.G + rr - tk * t.G;
-    bf16_t* op = (bf16_t*)a.out + (long)(t.s.t0 + tk) * a.out_token_stride + (long)hd * a.out_head_stride + d0;
+    bf16_t* op = (bf16_t*)a.out + (long)(t.s.t0 + tk) * a.out_token_stride + (long)hd * a.out_head_stride + lane * EPL;
     const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
-    for (int e = 0; e < EPT; e += 4) {
-        const float v[4] = {o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv};
-        store4_split(op + e, a.out_lo, v);
-    }
+    for (int e = 0; e < EPL; ++e) store_split(op + e, a.out_lo, o[e] * inv);
 }
 
 // ---------------------------------------------------------------------------------------------------------- host side
@@ -554,7 +570,7 @@ void launch_kv_attend(hipStream_t st, KvAttendArgs a, const KvAttendPlan& p) {
     a.split_len = p.split_len;
     const unsigned pairs = (unsigned)(a.b.n_seq * a.kv.nkv);
     // pairs vary fastest and are padded to the number of XCDs: all tiles and parts of a pair run on one XCD and share its L2
-    const dim3 grid((pairs + 7) / 8 * 8, (unsigned)p.tiles, (unsigned)p.splits), join(pairs * (unsigned)p.tiles, (unsigned)(p.tile_rows / 16));
+    const dim3 grid((pairs + 7) / 8 * 8, (unsigned)p.tiles, (unsigned)p.splits), join(pairs * (unsigned)p.tiles, (unsigned)(p.tile_rows / 4));
 #define QTTS_KV_ATTEND(FMT, DD)                                                                        \
     if (a.kv.format == FMT && a.kv.d == DD) {                                                          \
         if (p.tile_rows == 16) kv_launch(kv_attend_few_kernel<FMT, DD>, grid, dim3(256), st, a);       \

@@ -45,6 +45,7 @@ struct KvMoveArgs {         // write: k, v -> cache; read: cache -> k, v
     const void *k_in, *v_in;
     void *k_out, *v_out;
     long k_token_stride, k_head_stride, v_token_stride, v_head_stride;  // elements
+    int head_shift;          // set by the launchers
 };
 void launch_kv_write(hipStream_t st, int dtype, const KvMoveArgs& a);
 void launch_kv_read(hipStream_t st, int dtype, const KvMoveArgs& a);
@@ -70,6 +71,7 @@ struct KvAttendArgs {
 };
 // How a call is cut: row tiles (a row = one query head of one token; the rows of a sequence and kv head in token order), and
 // parts of the key range whose partial results a second launch joins.
+constexpr int KV_MAX_PARTS = 256;
 struct KvAttendPlan {
     int tile_rows;          // 16: one wave walks keys by itself; 128: four waves share the keys through LDS
     int tiles;              // row tiles a sequence and kv head can have

@@ -5,6 +5,7 @@
 
 namespace qtts {
 
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));  // register arrays of HIP's uint4 end in scratch memory
 
 // biased exponent of a block's scale from the largest |x| (as bits): see KvFormat.  448 = 1.75 2^8 and 127 = 1.984375 2^6.
@@ -46,20 +47,32 @@ __device__ __forceinline__ void kv_decode4(unsigned c, float scale, float* o) {
         o[2] = __builtin_amdgcn_cvt_f32_fp8((int)c, 2) * scale;
         o[3] = __builtin_amdgcn_cvt_f32_fp8((int)c, 3) * scale;
     } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = (float)((int)(c << (24 - 8 * i)) >> 24) * scale;
+        // the four codes stay one register until here: the compiler would carry them around the callers' loops as separate bytes
+        asm("" : "+v"(c));
+        // written with byte casts: the compiler takes a byte out, extends its sign and converts it in one instruction
+        o[0] = (float)(signed char)(c & 0xffu) * scale;
+        o[1] = (float)(signed char)((c >> 8) & 0xffu) * scale;
+        o[2] = (float)(signed char)((c >> 16) & 0xffu) * scale;
+        o[3] = (float)(signed char)(c >> 24) * scale;
     }
 }
-__device__ __forceinline__ unsigned pack_bf16(float a, float b) {
-    return (unsigned)f32_to_bf16_bits(a) | ((unsigned)f32_to_bf16_bits(b) << 16);
+__device__ __forceinline__ unsigned pack_bf16(float a, float b) {  // one conversion for both (round to nearest even)
+    typedef float f32x2_t __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
 }
 // eight codes -> eight bf16 in operand order, exact (see KvFormat)
 template <int FMT>
 __device__ __forceinline__ u32x4_t kv_decode8(unsigned c0, unsigned c1, float scale) {
-    float f[8];
-    kv_decode4<FMT>(c0, scale, f);
-    kv_decode4<FMT>(c1, scale, f + 4);
-    return u32x4_t{pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7])};
+    if constexpr (FMT == KV_E4M3) {  // one instruction converts, scales and packs two codes
+        const auto two = [&](bf16x2_t v) { return __builtin_bit_cast(unsigned, v); };
+        return u32x4_t{two(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c0, scale, false)), two(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c0, scale, true)),
+                       two(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c1, scale, false)), two(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c1, scale, true))};
+    } else {
+        float f[8];
+        kv_decode4<FMT>(c0, scale, f);
+        kv_decode4<FMT>(c1, scale, f + 4);
+        return u32x4_t{pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7])};
+    }
 }
 
 }  // namespace qtts

@@ -92,9 +92,9 @@ inline KvAttendPlan kv_attend_plan(const KvLayer& kv, const KvBatch& b, int nh, 
     const long span_tokens = std::min<long>(b.max_new, (p.tile_rows - 1) / (nh / kv.nkv) + 2);
     const long keys = std::max<long>(1, window ? std::min<long>(b.max_ctx, window + span_tokens + 63) : b.max_ctx);
     const long units = (long)b.n_seq * kv.nkv * p.tiles;
-    const long want = std::max<long>(1, 1024 / std::max<long>(units, 1));
+    const long want = std::max<long>(1, (p.tile_rows == 16 ? 1024 : 512) / std::max<long>(units, 1));
     const long most = std::max<long>(1, (keys + 511) / 512);
-    p.splits = (int)std::min<long>(std::min(want, most), 256);
+    p.splits = (int)std::min<long>(std::min(want, most), KV_MAX_PARTS);
     p.split_len = (int)(((keys + p.splits - 1) / p.splits + 127) / 128 * 128);
     if (p.splits > 1) p.ws_bytes = (size_t)units * p.splits * p.tile_rows * (kv.d + 2) * sizeof(float);
     return p;
