@@ -1,29 +1,24 @@
 // Writing keys and values into the paged cache and reading them back (gfx950), and the talker's projection pass that ends in it.
 //
-// Both directions are bound by the bytes they move; nothing is reused.  A lane owns 16 bytes of a row of the caller's tensor, so that
-// one access of a wave is contiguous there (64-byte pieces per lane cost the f32 read back half its rate: 26 us instead of 18 us for
-// 84 MB), 8 or 4 codes of the cache, and a quarter or an eighth of a block of 32 whose largest element goes round by lane swaps.  A
-// block of threads stays with one head while there are many tokens, so that its rows are neighbours in the cache's pages, and with
-// one token otherwise; a thread has four rows in flight.
+// Both directions are bound by the bytes they move; nothing is reused.  Writing, a lane owns 16 elements: loads may come in pieces (a
+// line's other pieces are in the cache by then), stores should not, and 16 codes leave as 16 bytes; two neighbouring lanes hold a
+// block of 32 and share its largest element with one lane swap.  Reading back, a lane owns 16 bytes of the caller's row, so that a
+// wave's store is contiguous (84 MB of f32: 26 us with 64-byte pieces per lane, 16 us so).  A thread has two or four rows in flight;
+// a block of threads covers as many heads as it has rows, so that it stays within neighbouring rows of the caller's tensor.
 #include "kv_device.hpp"
 
 #include <algorithm>
 
 namespace qtts {
 
-constexpr int KV_MOVE_UNROLL = 4;
+template <typename T, bool WRITE>
+constexpr int kv_move_elems() { return WRITE ? 16 : 16 / (int)sizeof(T); }  // elements a lane owns
+template <bool WRITE>
+constexpr int kv_move_rows() { return WRITE ? 2 : 4; }                      // rows a thread has in flight
 
 template <int CTRL>
 __device__ __forceinline__ unsigned dpp_max(unsigned v) {
     return max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false));
-}
-// largest value of the 4 or 8 neighbouring lanes that hold a block, left in all of them
-template <int LANES>
-__device__ __forceinline__ unsigned block_max(unsigned v) {
-    v = dpp_max<0xb1>(v);                          // quad_perm 1 0 3 2
-    v = dpp_max<0x4e>(v);                          // quad_perm 2 3 0 1
-    if constexpr (LANES == 8) v = dpp_max<0x141>(v);  // row_half_mirror
-    return v;
 }
 __device__ __forceinline__ void load_piece(const bf16_t* p, float (&x)[8]) { load8(p, x); }
 __device__ __forceinline__ void load_piece(const float* p, float (&x)[4]) {
@@ -34,6 +29,22 @@ __device__ __forceinline__ void load_piece(const bf16_t* p, float (&x)[4]) {
     const uint2 v = *reinterpret_cast<const uint2*>(p);
     x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xffff0000u);
     x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xffff0000u);
+}
+__device__ __forceinline__ void load_piece(const bf16_t* p, float (&x)[16]) {
+    float a[8], b[8];
+    load8(p, a);
+    load8(p + 8, b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { x[i] = a[i]; x[8 + i] = b[i]; }
+}
+__device__ __forceinline__ void load_piece(const float* p, float (&x)[16]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(x + 4 * i) = *reinterpret_cast<const float4*>(p + 4 * i);
+}
+__device__ __forceinline__ void store_piece(bf16_t* p, const float (&x)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 8)
+        *reinterpret_cast<u32x4_t*>(p + i) = u32x4_t{pack_bf16(x[i], x[i + 1]), pack_bf16(x[i + 2], x[i + 3]), pack_bf16(x[i + 4], x[i + 5]), pack_bf16(x[i + 6], x[i + 7])};
 }
 __device__ __forceinline__ void store_piece(bf16_t* p, const float (&x)[8]) {
     *reinterpret_cast<u32x4_t*>(p) = u32x4_t{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
@@ -46,7 +57,7 @@ __device__ __forceinline__ void store_piece(bf16_t* p, const float (&x)[4]) {
 // grid: x = sequence, y = tokens, z = (keys | values) x heads; a.head_shift: log2 of the heads a block covers
 template <typename T, int FMT, int D, bool WRITE>
 __global__ __launch_bounds__(256) void kv_move_kernel(KvMoveArgs a) {
-    constexpr int EPT = 16 / (int)sizeof(T), LPR = D / EPT, RPB = 256 / LPR, U = KV_MOVE_UNROLL;  // elements a lane owns, lanes per row, rows per pass
+    constexpr int EPT = kv_move_elems<T, WRITE>(), LPR = D / EPT, RPB = 256 / LPR, U = kv_move_rows<WRITE>();  // lanes per row, rows per pass
     const KvSeq s = kv_seq(a.b, blockIdx.x);
     const int zh = (int)gridDim.z >> 1, which = (int)blockIdx.z >= zh, sub = threadIdx.x % LPR;
     const int rib = threadIdx.x / LPR, g = (((int)blockIdx.z - (which ? zh : 0)) << a.head_shift) + (rib & ((1 << a.head_shift) - 1));
@@ -92,7 +103,7 @@ __global__ __launch_bounds__(256) void kv_move_kernel(KvMoveArgs a) {
                 unsigned m = 0;
 #pragma unroll
                 for (int e = 0; e < EPT; ++e) m = max(m, __float_as_uint(x[k][e]) & 0x7fffffffu);
-                if constexpr (FMT != KV_BF16) m = block_max<KV_BLOCK / EPT>(m);
+                if constexpr (FMT != KV_BF16) m = dpp_max<0xb1>(m);  // the other half of the block: lane ^ 1
                 if (page[k] < 0) continue;
                 row[k] = kv_row(a.kv, page[k], which, g, s.ctx - s.n + i);
                 if constexpr (FMT == KV_BF16) {
@@ -102,9 +113,10 @@ __global__ __launch_bounds__(256) void kv_move_kernel(KvMoveArgs a) {
                     const int ex = bad ? kv_bad_exp<FMT>() : kv_scale_exp<FMT>(m);
                     const float inv = __uint_as_float((unsigned)(254 - (bad ? 127 : ex)) << 23);
                     unsigned char* cp = a.kv.codes + row[k] * D + sub * EPT;
-                    const unsigned c0 = bad ? kv_bad_codes<FMT>() : kv_encode4<FMT>(x[k], inv);
-                    if constexpr (EPT == 8) *reinterpret_cast<uint2*>(cp) = make_uint2(c0, bad ? kv_bad_codes<FMT>() : kv_encode4<FMT>(x[k] + 4, inv));
-                    else *reinterpret_cast<unsigned*>(cp) = c0;
+                    u32x4_t c;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) c[e] = bad ? kv_bad_codes<FMT>() : kv_encode4<FMT>(x[k] + 4 * e, inv);
+                    *reinterpret_cast<u32x4_t*>(cp) = c;
                     if (sub % (KV_BLOCK / EPT) == 0) a.kv.scales[row[k] * (D / KV_BLOCK) + sub * EPT / KV_BLOCK] = (unsigned char)ex;
                 }
             } else if (i < s.n) {
@@ -121,10 +133,10 @@ __global__ __launch_bounds__(256) void kv_move_kernel(KvMoveArgs a) {
 template <bool WRITE>
 static void launch_kv_move(hipStream_t st, int dtype, KvMoveArgs a) {
     if (a.b.n_seq == 0 || a.b.n_tokens == 0 || a.b.max_new == 0) return;
-    const int rpb = 256 / (a.kv.d * (int)dtype_size(dtype) / 16);  // rows per pass
+    const int rpb = 256 / (a.kv.d / (WRITE ? 16 : 16 / (int)dtype_size(dtype)));  // rows per pass
     a.head_shift = 0;
     while ((2 << a.head_shift) <= rpb && (1 << a.head_shift) < a.kv.nkv) ++a.head_shift;
-    const long tokens = (long)(rpb >> a.head_shift) * KV_MOVE_UNROLL, heads = (a.kv.nkv + (1 << a.head_shift) - 1) >> a.head_shift;
+    const long tokens = (long)(rpb >> a.head_shift) * kv_move_rows<WRITE>(), heads = (a.kv.nkv + (1 << a.head_shift) - 1) >> a.head_shift;
     const dim3 grid((unsigned)a.b.n_seq, (unsigned)std::min<long>((a.b.max_new + tokens - 1) / tokens, 65535), (unsigned)(2 * heads));
 #define QTTS_KV_MOVE(T, FMT, DD) \
     if (a.kv.format == FMT && a.kv.d == DD) return kv_launch(kv_move_kernel<T, FMT, DD, WRITE>, grid, dim3(256), st, a);
