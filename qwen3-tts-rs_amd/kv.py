@@ -53,6 +53,11 @@ class KVCache:
         if format not in KV_FORMATS:
             raise QttsError(-1, f"KVCache: unknown format '{format}'. Available: {sorted(KV_FORMATS)}")
         import torch
+        self._torch = torch
+        self._f32, self._bf16 = torch.float32, torch.bfloat16
+        # the stream's handle without a Stream object around it (2 us of a call's 10) where torch has that
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        self._stream = (lambda: raw(int(device))) if raw else (lambda: torch.cuda.current_stream(self.device).cuda_stream)
         self.lib = _lib.load()
         self.layers, self.pages, self.page_tokens = int(layers), int(pages), int(page_tokens)
         self.kv_heads, self.head_dim, self.format = int(kv_heads), int(head_dim), format
@@ -109,7 +114,6 @@ class KVCache:
 
     # ------------------------------------------------------------------ calls
     def _check(self, what, layer, batch, t, heads, dtypes):
-        import torch
         if not 0 <= layer < self.layers:
             raise QttsError(-1, f"{what}: no such layer")
         if not isinstance(batch, KVBatch):
@@ -120,62 +124,58 @@ class KVCache:
             raise QttsError(-1, f"{what}: tensors must be on {self.device}")
         if t.dtype not in dtypes:
             raise QttsError(-1, f"{what}: dtype must be one of {[str(d) for d in dtypes]}")
-        if t.dim() != 3 or t.shape[0] != batch.n_tokens or t.shape[2] != self.head_dim or (heads and t.shape[1] != heads):
-            raise QttsError(-4, f"{what}: shape must be ({batch.n_tokens}, {heads or 'heads'}, {self.head_dim}), got {tuple(t.shape)}")
-        if t.numel() and t.stride(2) != 1:
+        shape = tuple(t.shape)
+        if len(shape) != 3 or shape[0] != batch.n_tokens or shape[2] != self.head_dim or (heads and shape[1] != heads):
+            raise QttsError(-4, f"{what}: shape must be ({batch.n_tokens}, {heads or 'heads'}, {self.head_dim}), got {shape}")
+        if t.stride(2) != 1 and t.numel():
             raise QttsError(-1, f"{what}: the elements of a head must be contiguous")
-        if t.requires_grad and torch.is_grad_enabled():
+        if t.requires_grad and self._torch.is_grad_enabled():
             raise QttsError(-1, f"{what}: inference only, the tensor requires a gradient")
 
-    def _rows(self, k, v):
-        r = _lib.KvRows(k.data_ptr(), v.data_ptr(), QTTS_F32 if k.element_size() == 4 else QTTS_BF16, k.stride(0), k.stride(1), v.stride(0),
+    def _move(self, call, layer, batch, k, v):
+        r = _lib.KvRows(k.data_ptr(), v.data_ptr(), QTTS_F32 if k.dtype == self._f32 else QTTS_BF16, k.stride(0), k.stride(1), v.stride(0),
                         v.stride(1))
-        return r, C.addressof(r)
-
-    def _stream(self):
-        import torch
-        return torch.cuda.current_stream(self.device).cuda_stream
+        check(call(self._kv, layer, batch._ptr, C.addressof(r), self._stream()))
 
     def write(self, layer: int, batch: KVBatch, k, v) -> None:
         """Holds the batch's tokens: k, v (n_tokens, kv_heads, head_dim), f32 or bf16."""
-        import torch
-        self._check("KVCache.write", layer, batch, k, self.kv_heads, (torch.bfloat16, torch.float32))
+        self._check("KVCache.write", layer, batch, k, self.kv_heads, (self._bf16, self._f32))
         self._check("KVCache.write", layer, batch, v, self.kv_heads, (k.dtype,))
-        r, p = self._rows(k, v)
-        check(self.lib.qtts_kv_write(self._kv, layer, batch._ptr, p, self._stream()))
+        self._move(self.lib.qtts_kv_write, layer, batch, k, v)
 
     def read(self, layer: int, batch: KVBatch, dtype=None, out=None):
         """The batch's tokens as they are held: (k, v), f32 or bf16 (the default); with new = ctx whole sequences.  out: a (k, v) pair
         to fill (rows behind the last sequence stay as they are)."""
-        import torch
         if out is None:
-            shape = (batch.n_tokens, self.kv_heads, self.head_dim)
-            out = tuple(torch.empty(shape, dtype=dtype or torch.bfloat16, device=self.device) for _ in range(2))
+            if not isinstance(batch, KVBatch):
+                raise QttsError(-1, "KVCache.read: not a KVBatch")
+            k = self._torch.empty((batch.n_tokens, self.kv_heads, self.head_dim), dtype=dtype or self._bf16, device=self.device)
+            out = k, self._torch.empty_like(k)
         k, v = out
-        self._check("KVCache.read", layer, batch, k, self.kv_heads, (torch.bfloat16, torch.float32) if dtype is None else (dtype,))
+        self._check("KVCache.read", layer, batch, k, self.kv_heads, (self._bf16, self._f32) if dtype is None else (dtype,))
         self._check("KVCache.read", layer, batch, v, self.kv_heads, (k.dtype,))
-        r, p = self._rows(k, v)
-        check(self.lib.qtts_kv_read(self._kv, layer, batch._ptr, p, self._stream()))
+        if k.dtype != self._bf16 and k.dtype != self._f32:
+            raise QttsError(-1, "KVCache.read: dtype must be float32 or bfloat16")
+        self._move(self.lib.qtts_kv_read, layer, batch, k, v)
         return k, v
 
     def attend(self, layer: int, batch: KVBatch, q, scale: Optional[float] = None, window: int = 0, out=None):
         """softmax(scale q k^T) v of the batch's tokens over what the cache holds for their sequences: q (n_tokens, heads, head_dim)
         bf16, heads a multiple of kv_heads; scale defaults to head_dim ** -0.5.  A token sees the positions up to its own, with a
         window the last `window` of them.  The tokens' own keys and values have been written before."""
-        import torch
-        self._check("KVCache.attend", layer, batch, q, 0, (torch.bfloat16,))
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-        else:
-            self._check("KVCache.attend: out", layer, batch, out, q.shape[1], (torch.bfloat16,))
+        self._check("KVCache.attend", layer, batch, q, 0, (self._bf16,))
         heads, window = q.shape[1], min(int(window), 0x7fffffff)
+        if out is None:
+            out = self._torch.empty_like(q, memory_format=self._torch.contiguous_format)
+        else:
+            self._check("KVCache.attend: out", layer, batch, out, heads, (self._bf16,))
         shape = (self.kv_heads, self.head_dim, heads, window)
         nbytes = batch._ws.get(shape)
         if nbytes is None:
             n = C.c_int64(0)
             check(self.lib.qtts_kv_attend_workspace(self._kv, batch._ptr, heads, window, C.byref(n)))
             nbytes = batch._ws[shape] = n.value
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
+        ws = self._torch.empty(nbytes, dtype=self._torch.uint8, device=self.device) if nbytes else None
         a = _lib.KvAttendArgs(q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), heads,
                               self.head_dim ** -0.5 if scale is None else scale, window, ws.data_ptr() if nbytes else None, nbytes)
         check(self.lib.qtts_kv_attend(self._kv, layer, batch._ptr, C.addressof(a), self._stream()))
