@@ -92,8 +92,11 @@ inline KvAttendPlan kv_attend_plan(const KvLayer& kv, const KvBatch& b, int nh, 
     const long span_tokens = std::min<long>(b.max_new, (p.tile_rows - 1) / (nh / kv.nkv) + 2);
     const long keys = std::max<long>(1, window ? std::min<long>(b.max_ctx, window + span_tokens + 63) : b.max_ctx);
     const long units = (long)b.n_seq * kv.nkv * p.tiles;
-    const long want = std::max<long>(1, (p.tile_rows == 16 ? 1024 : 512) / std::max<long>(units, 1));
-    const long most = std::max<long>(1, (keys + 511) / 512);
+    // Two blocks a CU fill it for either kernel, and a part of fewer than 256 keys is mostly start and join.  Measured with 16-row tiles, target
+    // 512 / 768 / 1024 blocks: 12 x 30011 int8 keys 124 / 131 / 140 us, 32 x 2047 with five tokens 32.2 / 30.6 / 34.0 us, 7 x 20011 bf16
+    // keys 23.2 / 26.4 / 26.5 us; parts of at least 512 keys: 24.8 us for the last.
+    const long want = std::max<long>(1, 512 / std::max<long>(units, 1));
+    const long most = std::max<long>(1, (keys + 255) / 256);
     p.splits = (int)std::min<long>(std::min(want, most), KV_MAX_PARTS);
     p.split_len = (int)(((keys + p.splits - 1) / p.splits + 127) / 128 * 128);
     if (p.splits > 1) p.ws_bytes = (size_t)units * p.splits * p.tile_rows * (kv.d + 2) * sizeof(float);
