@@ -270,7 +270,7 @@ __global__ __launch_bounds__(256, 3) void kv_attend_few_kernel(KvAttendArgs a) {
         for (int e = 0; e < EPT; ++e) o[e] += wt * Os[(w * 16 + orow) * LDO + d0 + e];
     }
     if (t.parts > 1) {
-        const size_t u = ((size_t)(pair * a.tiles + blockIdx.y) * a.splits + blockIdx.z) * 16 + orow;
+        const size_t u = ((size_t)(pair * a.tiles + blockIdx.y) * a.splits + blockIdx.z) * 16 + orow;  // slot
         float* po = a.ws + u * D + d0;
 #pragma unroll
         for (int e = 0; e < EPT; e += 4) *reinterpret_cast<float4*>(po + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
@@ -296,11 +296,11 @@ template <int FMT, int D>
 __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) {
     constexpr bool Q8 = FMT != KV_BF16;
     constexpr int KB = 64;
+    constexpr int LDK = D + 8;    // K rows 4 banks apart: 16 lanes' 16-byte reads hit every bank once
+    constexpr int LDV = D + 32;   // V rows 16 banks apart (modulo 64): the four rows of a transposing read share no bank
     constexpr int NS = D / 16, NDT = D / 32;          // contraction steps of K Q^T; 32-column tiles of the output
     constexpr int EPP = Q8 ? 16 : 8, PPR = D / EPP;   // elements per 16-byte piece of the cache, pieces per row
     constexpr int KPW = 64 / PPR, NP = KB / (4 * KPW);  // keys a wave stages at once, passes per block of keys
-    constexpr int LDK = D + 8;    // K rows 4 banks apart: 16 lanes' 16-byte reads hit every bank once
-    constexpr int LDV = D + 32;   // V rows 16 banks apart (modulo 64): the four rows of a transposing read share no bank
     __shared__ __attribute__((aligned(16))) u16 Ks[KB * LDK];
     __shared__ __attribute__((aligned(16))) u16 Vs[KB * LDV];
     __shared__ int sh_bad;
@@ -341,36 +341,37 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
     unsigned ksc[NP], vsc[NP];
     const int krow = lane / PPR, pc = lane % PPR;
     constexpr unsigned ROWB = Q8 ? D : 2 * D;  // bytes of a head row
-    const unsigned loff = krow * ROWB + pc * 16, lsoff = krow * (D / KV_BLOCK) + pc / 2;
-    auto load = [&](int kb, const int (&pg)[4]) {
+    // Lanes 0 .. 3 (modulo 4) work out where a block's four groups of 16 keys start and hand it round: as scalars of the loop these are a
+    // hundred instructions a block.  A hole is read as page 0: in bounds, and what it holds is masked.
+    const unsigned long page_bytes = ((unsigned long)a.kv.nkv << a.kv.page_shift) * (2 * ROWB);
+    const unsigned head_bytes = ((unsigned)t.g << a.kv.page_shift) * ROWB;
+    const unsigned koff = ((wave * KPW) & 15) * ROWB + krow * ROWB + pc * 16, voff = koff + (unsigned)(page_bytes >> 1);
+    int pv = -1;
+    unsigned holes = 0, hole = 0;  // bit i: group i of the block that travels, of the block in the images
+    auto load = [&](int kb) {      // pv: the block's pages
+        holes = (unsigned)__ballot(pv < 0) & 15u;
+        const unsigned long ga = (unsigned long)max(pv, 0) * page_bytes + head_bytes + ((kb + 16 * (lane & 3)) & ((1 << a.kv.page_shift) - 1)) * ROWB;
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
-            const int k0 = (n * 4 + wave) * KPW;  // the wave's first key of this pass; all of them in one group of 16
-            const size_t kr = kv_row(a.kv, max(pg[k0 >> 4], 0), 0, t.g, kb + k0), vr = kr + ((size_t)a.kv.nkv << a.kv.page_shift);
-            kreg[n] = *reinterpret_cast<const u32x4_t*>(a.kv.codes + kr * ROWB + loff);
-            vreg[n] = *reinterpret_cast<const u32x4_t*>(a.kv.codes + vr * ROWB + loff);
-            if constexpr (Q8) {
-                ksc[n] = (a.kv.scales + kr * (D / KV_BLOCK))[lsoff];
-                vsc[n] = (a.kv.scales + vr * (D / KV_BLOCK))[lsoff];
+            const int gi = ((n * 4 + wave) * KPW) >> 4;  // group of the wave's keys in this pass
+            const unsigned long at = ((unsigned long)(unsigned)__builtin_amdgcn_readlane((int)(ga >> 32), gi) << 32) | (unsigned)__builtin_amdgcn_readlane((int)ga, gi);
+            kreg[n] = *reinterpret_cast<const u32x4_t*>(a.kv.codes + at + koff);
+            vreg[n] = *reinterpret_cast<const u32x4_t*>(a.kv.codes + at + voff);
+            if constexpr (Q8) {  // a scale byte per 32 code bytes
+                ksc[n] = (a.kv.scales + (at >> 5))[koff / KV_BLOCK];
+                vsc[n] = (a.kv.scales + (at >> 5))[voff / KV_BLOCK];
             }
         }
     };
-    // lanes 0 .. 3 (modulo 4) have the pages of the next block's four groups of 16 keys
-    int pv = -1, pg[4] = {-1, -1, -1, -1};
-    auto take = [&]() {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) pg[i] = __builtin_amdgcn_readlane(pv, i);
-    };
     if (t.s0 < t.s1) {
         pv = kv_page16(a, t, t.s0 + 16 * (lane & 3));
-        take();
-        load(t.s0, pg);
+        load(t.s0);
         pv = kv_page16(a, t, t.s0 + KB + 16 * (lane & 3));
     }
     if (threadIdx.x == 0) sh_bad = -1;
     for (int kb = t.s0; kb < t.s1; kb += KB) {
         const bool mixed = kb + KB - 1 > t.p0 || (a.window && kb <= t.p1 - a.window);
-        const bool edge = mixed || kb < t.k_begin || kb + KB > t.s1 || (pg[0] | pg[1] | pg[2] | pg[3]) < 0;
+        const bool edge = mixed || kb < t.k_begin || kb + KB > t.s1 || holes;
         __syncthreads();  // every wave is done with the previous image
         bool bad = false;
 #pragma unroll
@@ -389,7 +390,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
                 w[0] = vreg[n];
             }
             if (edge) {
-                const bool in = kb + key >= t.k_begin && kb + key < t.s1 && pg[k0 >> 4] >= 0;
+                const bool in = kb + key >= t.k_begin && kb + key < t.s1 && !((holes >> (k0 >> 4)) & 1u);
 #pragma unroll
                 for (int h = 0; h < (Q8 ? 2 : 1); ++h) {
                     w[h] = keep(w[h], in);
@@ -400,9 +401,8 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
             for (int h = 0; h < (Q8 ? 2 : 1); ++h) *reinterpret_cast<u32x4_t*>(Vs + key * LDV + pc * EPP + 8 * h) = w[h];
         }
         if (bad) sh_bad = kb;
-        const int pcur[4] = {pg[0], pg[1], pg[2], pg[3]};
-        take();
-        load(kb + KB, pg);  // behind the part: page 0, not used
+        hole = holes;
+        load(kb + KB);  // behind the part: page 0, not used
         pv = kv_page16(a, t, kb + 2 * KB + 16 * (lane & 3));
         __syncthreads();
         if (mixed && sh_bad == kb) {
@@ -441,14 +441,14 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
                 s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8_t*>(kp + 16 * j), q[j], s[kt], 0, 0, 0);
         }
         // s[kt][i] = key kb + 32 kt + 8 (i / 4) + 4 hf + i % 4 of this lane's row
-        const bool whole = kb + KB - 1 <= wp0 && !(a.window && kb <= wp1 - a.window) && kb + KB <= t.s1 && (pcur[0] | pcur[1] | pcur[2] | pcur[3]) >= 0;
+        const bool whole = kb + KB - 1 <= wp0 && !(a.window && kb <= wp1 - a.window) && kb + KB <= t.s1 && !hole;
         if (!whole) {
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int key = kb + 32 * kt + 8 * (i >> 2) + 4 * hf + (i & 3);
-                    const bool see = key >= klo && key <= pos && key < t.s1 && pcur[2 * kt + (i >> 3)] >= 0;
+                    const bool see = key >= klo && key <= pos && key < t.s1 && !((hole >> (2 * kt + (i >> 3))) & 1u);
                     s[kt][i] = see ? s[kt][i] : -INFINITY;
                 }
         }
@@ -514,10 +514,11 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
 
 // ------------------------------------------------------------------------------------------------ joining the parts
 // One wave per row: its lanes take the parts' maxima and sums (64 at a time) and turn them into weights; then each lane adds up its
-// D / 64 columns of the parts' outputs with eight loads in flight.
-template <int TR, int D>
-__global__ __launch_bounds__(256) void kv_attend_join_kernel(KvAttendArgs a) {
-    constexpr int EPL = D / 64;
+// D / 64 columns of the parts' outputs with eight loads in flight: 5 us for 73 parts of 56 rows, where one thread an element and all parts in a
+// row of loads took 19 us and the kernel below takes 11 us.
+template <int D>
+__global__ __launch_bounds__(256) void kv_attend_join_few_kernel(KvAttendArgs a) {
+    constexpr int TR = 16, EPL = D / 64;
     typedef float vec_t __attribute__((ext_vector_type(EPL)));
     const int unit = blockIdx.x, pair = unit / a.tiles, tile = unit - pair * a.tiles;
     const KvTile t = kv_tile<TR>(a, pair, tile, 0);
@@ -561,6 +562,52 @@ __global__ __launch_bounds__(256) void kv_attend_join_kernel(KvAttendArgs a) {
     for (int e = 0; e < EPL; ++e) store_split(op + e, a.out_lo, o[e] * inv);
 }
 
+// Tiles of 128 rows have few parts and many rows: D / 4 lanes a row, each with 16 bytes of it, O = sum_s 2^(m_s - M) O_s over
+// sum_s 2^(m_s - M) l_s, four parts' loads in flight.  Bound by the partial results' bytes (20 us for 60 MB; a wave per row 34 us).
+template <int D>
+__global__ __launch_bounds__(256) void kv_attend_join_tile_kernel(KvAttendArgs a) {
+    constexpr int TR = 128, LPR = D / 4, RPB = 256 / LPR;
+    const int unit = blockIdx.x, pair = unit / a.tiles, tile = unit - pair * a.tiles;
+    const KvTile t = kv_tile<TR>(a, pair, tile, 0);
+    const int trow = (int)blockIdx.y * RPB + threadIdx.x / LPR, rr = t.row0 + trow, d0 = threadIdx.x % LPR * 4;
+    if (!t.live || t.parts == 1 || rr >= t.rows) return;
+    const size_t u = (size_t)unit * a.splits * TR + trow;
+    const float* ml = a.ws + (size_t)a.b.n_seq * a.kv.nkv * a.tiles * a.splits * TR * D + u * 2;
+    const float* po = a.ws + u * D + d0;
+    float M = -INFINITY, L = 0.f;
+    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < t.parts; s += 4) {
+        float m[4], l[4];
+        f32x4_t v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const size_t q = (size_t)min(s + k, t.parts - 1) * TR;
+            const float2 x = *reinterpret_cast<const float2*>(ml + q * 2);
+            m[k] = s + k < t.parts ? x.x : -INFINITY;  // a part that is not there weighs nothing
+            l[k] = x.y;
+            v[k] = *reinterpret_cast<const f32x4_t*>(po + q * D);
+        }
+        const float mn = fmaxf(M, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
+        const float ref = mn == -INFINITY ? 0.f : mn;
+        const float alpha = __builtin_amdgcn_exp2f(M - ref);
+        L *= alpha;
+        o *= alpha;
+        M = mn;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float w = __builtin_amdgcn_exp2f(m[k] - ref);
+            L += s + k < t.parts ? w * l[k] : 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] += s + k < t.parts ? w * v[k][e] : 0.f;
+        }
+    }
+    const int tk = rr / t.G, hd = t.g * t.G + rr - tk * t.G;
+    bf16_t* op = (bf16_t*)a.out + (long)(t.s.t0 + tk) * a.out_token_stride + (long)hd * a.out_head_stride + d0;
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const float r[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+    store4_split(op, a.out_lo, r);
+}
+
 // ---------------------------------------------------------------------------------------------------------- host side
 void launch_kv_attend(hipStream_t st, KvAttendArgs a, const KvAttendPlan& p) {
     if (a.b.n_seq == 0 || a.b.n_tokens == 0) return;
@@ -570,16 +617,18 @@ void launch_kv_attend(hipStream_t st, KvAttendArgs a, const KvAttendPlan& p) {
     a.split_len = p.split_len;
     const unsigned pairs = (unsigned)(a.b.n_seq * a.kv.nkv);
     // pairs vary fastest and are padded to the number of XCDs: all tiles and parts of a pair run on one XCD and share its L2
-    const dim3 grid((pairs + 7) / 8 * 8, (unsigned)p.tiles, (unsigned)p.splits), join(pairs * (unsigned)p.tiles, (unsigned)(p.tile_rows / 4));
-#define QTTS_KV_ATTEND(FMT, DD)                                                                        \
-    if (a.kv.format == FMT && a.kv.d == DD) {                                                          \
-        if (p.tile_rows == 16) kv_launch(kv_attend_few_kernel<FMT, DD>, grid, dim3(256), st, a);       \
-        else kv_launch(kv_attend_tile_kernel<FMT, DD>, grid, dim3(256), st, a);                        \
-        if (p.splits > 1) {                                                                            \
-            if (p.tile_rows == 16) kv_launch(kv_attend_join_kernel<16, DD>, join, dim3(256), st, a);   \
-            else kv_launch(kv_attend_join_kernel<128, DD>, join, dim3(256), st, a);                    \
-        }                                                                                              \
-        return;                                                                                        \
+    const dim3 grid((pairs + 7) / 8 * 8, (unsigned)p.tiles, (unsigned)p.splits);
+    const dim3 join(pairs * (unsigned)p.tiles, p.tile_rows == 16 ? 4u : (unsigned)a.kv.d / 8u);
+#define QTTS_KV_ATTEND(FMT, DD)                                                                          \
+    if (a.kv.format == FMT && a.kv.d == DD) {                                                            \
+        if (p.tile_rows == 16) {                                                                         \
+            kv_launch(kv_attend_few_kernel<FMT, DD>, grid, dim3(256), st, a);                            \
+            if (p.splits > 1) kv_launch(kv_attend_join_few_kernel<DD>, join, dim3(256), st, a);          \
+        } else {                                                                                         \
+            kv_launch(kv_attend_tile_kernel<FMT, DD>, grid, dim3(256), st, a);                           \
+            if (p.splits > 1) kv_launch(kv_attend_join_tile_kernel<DD>, join, dim3(256), st, a);         \
+        }                                                                                                \
+        return;                                                                                          \
     }
     QTTS_KV_ATTEND(KV_BF16, 64)
     QTTS_KV_ATTEND(KV_E4M3, 64)

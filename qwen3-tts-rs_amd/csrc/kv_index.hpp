@@ -92,12 +92,29 @@ inline KvAttendPlan kv_attend_plan(const KvLayer& kv, const KvBatch& b, int nh, 
     const long span_tokens = std::min<long>(b.max_new, (p.tile_rows - 1) / (nh / kv.nkv) + 2);
     const long keys = std::max<long>(1, window ? std::min<long>(b.max_ctx, window + span_tokens + 63) : b.max_ctx);
     const long units = (long)b.n_seq * kv.nkv * p.tiles;
-    // Two blocks a CU fill it for either kernel, and a part of fewer than 256 keys is mostly start and join.  Measured with 16-row tiles, target
-    // 512 / 768 / 1024 blocks: 12 x 30011 int8 keys 124 / 131 / 140 us, 32 x 2047 with five tokens 32.2 / 30.6 / 34.0 us, 7 x 20011 bf16
-    // keys 23.2 / 26.4 / 26.5 us; parts of at least 512 keys: 24.8 us for the last.
-    const long want = std::max<long>(1, 512 / std::max<long>(units, 1));
-    const long most = std::max<long>(1, (keys + 255) / 256);
-    p.splits = (int)std::min<long>(std::min(want, most), KV_MAX_PARTS);
+    p.splits = 1;
+    if (p.tile_rows == 16) {
+        // Two blocks a CU fill it, and a part of fewer than 256 keys is mostly start and join.  Measured with targets of 512 / 768 / 1024
+        // blocks: 12 x 30011 int8 keys 124 / 131 / 140 us, 32 x 2047 with five tokens 32.2 / 30.6 / 34.0 us, 7 x 20011 bf16 keys 23.2 / 26.4 /
+        // 26.5 us; parts of at least 512 keys: 24.8 us for the last.
+        const long want = std::max<long>(1, 512 / std::max<long>(units, 1)), most = std::max<long>(1, (keys + 255) / 256);
+        p.splits = (int)std::min<long>(std::min(want, most), KV_MAX_PARTS);
+    } else {
+        // 512 blocks run at once.  Parts are worth their join where without them the last round of blocks is mostly empty: the fewest
+        // parts that fill it to nine tenths, else the best.  Measured: 384 tiles of up to 15013 e4m3 keys 508 us in one part, 400 us in four;
+        // 256 tiles of 20480 keys 564 / 404 / 420 us in 1 / 2 / 8 parts; where the rounds are full (2 x 4096 tokens, 1024 tiles) parts cost more
+        // than they give (185 us, 217 us in two).
+        double best = 0;
+        for (int s = 1; s <= KV_MAX_PARTS && best < 0.9; ++s) {
+            const long blocks = units * s;
+            if (s > 1 && keys < (blocks > 512 ? 1024L : 256L) * s) break;
+            const double fill = (double)blocks / (double)((blocks + 511) / 512 * 512);
+            if (fill > best) {
+                best = fill;
+                p.splits = s;
+            }
+        }
+    }
     p.split_len = (int)(((keys + p.splits - 1) / p.splits + 127) / 128 * 128);
     if (p.splits > 1) p.ws_bytes = (size_t)units * p.splits * p.tile_rows * (kv.d + 2) * sizeof(float);
     return p;
