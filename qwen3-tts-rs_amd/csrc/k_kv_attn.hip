@@ -432,14 +432,15 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
 
         f32x16_t s[2];
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
+        for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[kt][i] = 0.f;
-            const u16* kp = Ks + (kt * 32 + r) * LDK + 8 * hf;
+        const u16* kp = Ks + r * LDK + 8 * hf;
 #pragma unroll
-            for (int j = 0; j < NS; ++j)
-                s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8_t*>(kp + 16 * j), q[j], s[kt], 0, 0, 0);
-        }
+        for (int j = 0; j < NS; ++j)
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+                s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8_t*>(kp + kt * 32 * LDK + 16 * j), q[j], s[kt], 0, 0, 0);
         // s[kt][i] = key kb + 32 kt + 8 (i / 4) + 4 hf + i % 4 of this lane's row
         const bool whole = kb + KB - 1 <= wp0 && !(a.window && kb <= wp1 - a.window) && kb + KB <= t.s1 && !hole;
         if (!whole) {
