@@ -292,10 +292,10 @@ typedef struct {
  * The host integers bound what the device arrays hold: lengths beyond them are cut, so that no content of the arrays leads outside
  * a buffer. */
 typedef struct {
-    int n_seq;
+    int n_seq;                /* n_seq * kv_heads below 2^23 */
     int n_tokens;             /* rows of the call's tensors */
     int max_new;              /* at least every sequence's n */
-    int max_ctx;              /* at least every ctx_len; at most max_pages * page_tokens */
+    int max_ctx;              /* at least every ctx_len; at most max_pages * page_tokens and 2^29 */
     int max_pages;            /* columns of page_table */
     const int32_t* q_start;   /* [n_seq + 1], rising, q_start[n_seq] <= n_tokens */
     const int32_t* ctx_len;   /* [n_seq], n at least */
@@ -328,7 +328,7 @@ int qtts_kv_write(qtts_kv_cache* kv, int layer, const qtts_kv_batch* batch, cons
 /* Reads the batch's tokens back (the values they are held as); with n = ctx_len whole sequences. */
 int qtts_kv_read(qtts_kv_cache* kv, int layer, const qtts_kv_batch* batch, const qtts_kv_rows* rows, void* stream);
 /* out = softmax(scale q k^T) v of the batch's tokens over the held keys and values: a token at position p sees positions
- * p-window+1 .. p (0 .. p without a window); a row that sees nothing is zero.  The tokens' own keys and values have been
+ * p-window+1 .. p (0 .. p without a window); a row that sees nothing, or whose every score is -infinity, is zero.  The tokens' own keys and values have been
  * written before.  The workspace size depends on the batch's host integers only. */
 int qtts_kv_attend_workspace(qtts_kv_cache* kv, const qtts_kv_batch* batch, int n_heads, int window, int64_t* bytes);
 int qtts_kv_attend(qtts_kv_cache* kv, int layer, const qtts_kv_batch* batch, const qtts_kv_attend_args* args, void* stream);

@@ -10,7 +10,7 @@
 //   O^T = V^T P^T the score registers are the B operand as they stand once the keys of a matrix step are numbered in the order in
 //                 which the lanes hold them; V^T comes out of a row-major LDS image by transposing reads.
 // Rounding: K, V and Q enter exactly (bf16, or codes times a power of two).  P is rounded to bf16 for the second product, at most
-// 2^-9 relative per term, of the order of the output's own rounding; l is summed from the unrounded f32 values.
+// 2^-8 relative per term, as the output itself is afterwards; l is summed from the unrounded f32 values.
 // Key ranges of few rows are cut into parts (KvAttendPlan) whose (m, l, O) a second launch joins.
 // A masked key may hold anything: its score is replaced, and its V row meets the products as zero.  Where some rows of a tile see a key
 // and others do not, a non-finite V element is taken out of the products and added to the rows that see it one by one.

@@ -82,8 +82,8 @@ static KvBatch check_batch(const KvCache& k, int layer, const qtts_kv_batch& b) 
     QTTS_CHECK(b.n_seq == 0 || (b.q_start && b.ctx_len), ERR_BAD_ARG, "kv cache: the batch lacks q_start or ctx_len");
     QTTS_CHECK(b.n_seq == 0 || b.max_pages == 0 || b.page_table, ERR_BAD_ARG, "kv cache: the batch lacks a page table");
     QTTS_CHECK((int64_t)b.max_ctx <= (int64_t)b.max_pages * k.page_tokens, ERR_SHAPE, "kv cache: max_ctx exceeds max_pages pages");
-    QTTS_CHECK(b.max_ctx <= 1 << 30 && b.max_new <= 1 << 24 && b.n_tokens <= 1 << 30, ERR_SHAPE, "kv cache: batch too large");
-    QTTS_CHECK((int64_t)b.n_seq * k.nkv <= 1 << 30, ERR_SHAPE, "kv cache: too many sequences");
+    QTTS_CHECK(b.max_ctx <= 1 << 29 && b.max_new <= 1 << 24 && b.n_tokens <= 1 << 30, ERR_SHAPE, "kv cache: batch too large");
+    QTTS_CHECK((int64_t)b.n_seq * k.nkv < 1 << 23, ERR_SHAPE, "kv cache: too many sequences");
     return KvBatch{b.n_seq, b.n_tokens, b.max_new, b.max_ctx, b.q_start, b.ctx_len, 1, 0, nullptr};
 }
 

@@ -412,6 +412,93 @@ def test_captured_steps():
             assert torch.equal(w["out"], w["cache"].attend(0, w["b"], w["bufs"][2]))  # eager, between the replays
 
 
+def test_two_threads():
+    """Two host threads, each with a stream and batches of its own, on one cache."""
+    import threading
+    d, page = 64, 16
+    cache = KVCache(pages=64, kv_heads=2, head_dim=d, format="e4m3", page_tokens=page)
+    ctx = [300, 45]
+    table = torch.arange(38, dtype=torch.int32, device="cuda").view(2, 19)
+    data = [[rand((sum(ctx), 2, d), 10 * i + j) for j in range(2)] + [rand((2, 6, d), 10 * i + 5)] for i in range(2)]
+    tables = [table, torch.stack([torch.arange(38, 57), torch.cat([torch.arange(57, 60), torch.full((16,), -1)])]).to(torch.int32).cuda()]
+    outs, errors = [None, None], []
+    torch.cuda.synchronize()
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    cache.write(0, cache.batch(ctx, ctx, tables[i]), data[i][0], data[i][1])
+                    outs[i] = cache.attend(0, cache.batch([1, 1], ctx, tables[i]), data[i][2])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001 - reported by the test
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for i in range(2):
+        check_attend(outs[i], data[i][2], data[i][0], data[i][1], [1, 1], ctx, "e4m3", d ** -0.5)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_many_sequences_and_output_over_the_queries(new):
+    """1500 sequences of a few tokens; the output takes the queries' place."""
+    d, page, n = 64, 16, 1500
+    ctx = [new + b % 7 for b in range(n)]
+    table, pages = table_of(ctx, page)
+    cache = KVCache(pages=pages, kv_heads=1, head_dim=d, format="int8", page_tokens=page)
+    k, v, q = rand((sum(ctx), 1, d), 1), rand((sum(ctx), 1, d), 2), rand((n * new, 2, d), 3)
+    cache.write(0, cache.batch(ctx, ctx, table), k, v)
+    b = cache.batch([new] * n, ctx, table)
+    out = cache.attend(0, b, q)
+    place = q.clone()
+    cache.attend(0, b, place, out=place)
+    assert torch.equal(out, place)
+    some = list(range(0, n, 97))
+    pick = lambda x, lens: torch.cat([split(x, lens)[i] for i in some])  # noqa: E731
+    check_attend(pick(out, [new] * n), pick(q, [new] * n), pick(k, ctx), pick(v, ctx), [new] * len(some), [ctx[i] for i in some], "int8", d ** -0.5)
+
+
+@pytest.mark.parametrize("heads", [1, 40])
+def test_scores_that_are_not_finite(heads):
+    """Overflowing scores: +infinity makes the row NaN, -infinity leaves the key without weight."""
+    d, page, ctx = 64, 16, 70
+    table, pages = table_of([ctx], page)
+    cache = KVCache(pages=pages, kv_heads=1, head_dim=d, page_tokens=page)
+    k, v, q = rand((ctx, 1, d), 1), rand((ctx, 1, d), 2), rand((2, heads, d), 3)
+    q[:, :, 0] = 1e38
+    k[:, :, 0] = 0
+    k[3, 0, 0] = -1e38                     # -infinity for both rows
+    cache.write(0, cache.batch([ctx], [ctx], table), k, v)
+    b = cache.batch([2], [ctx], table)
+    check_attend(cache.attend(0, b, q), q, k[:, :, :], v, [2], [ctx], "bf16", d ** -0.5)
+    k[ctx - 1, 0, 0] = 1e38                # +infinity for the last row only
+    cache.write(0, cache.batch([ctx], [ctx], table), k, v)
+    out = cache.attend(0, b, q)
+    assert out[1].isnan().all() and out[0].isfinite().all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_wide_tiles_in_parts_with_holes_and_a_window(fmt):
+    """Row tiles whose keys are walked in parts (few kv heads, long contexts), ragged, with holes, with and without a window."""
+    d, page, heads, kv = 128, 64, 6, 2
+    ctx, new = [2600, 900, 70], [70, 45, 70]
+    table, pages = table_of(ctx, page)
+    cache = KVCache(pages=pages, kv_heads=kv, head_dim=d, format=fmt, page_tokens=page)
+    k, v, q = rand((sum(ctx), kv, d), 1), rand((sum(ctx), kv, d), 2), rand((sum(new), heads, d), 3)
+    cache.write(0, cache.batch(ctx, ctx, table), k, v)
+    table[0, 3], table[0, 40], table[1, 0] = -1, pages, -5
+    holes = [set(range(192, 256)) | set(range(2560, 2600)), set(range(64)), set()]
+    b = cache.batch(new, ctx, table)
+    assert workspace(cache, b, heads) > 0
+    for window in (0, 1700):
+        check_attend(cache.attend(0, b, q, window=window), q, k, v, new, ctx, fmt, d ** -0.5, window, holes)
+
+
 # ------------------------------------------------------------------------------------------------------------ refusals
 def test_refusals():
     d = 64

@@ -26,6 +26,12 @@ def hold(bind):
     set_top(0.0)
 
 
+def _icl_request(golden, ref):
+    from qwen3_tts_rs_amd import GenerationRequest
+    return GenerationRequest(text_ids=golden["text_ids"], language="english", speaker_embed=golden["xvector"], ref_codes=ref,
+                             ref_text_ids=golden["ref_text_ids"], non_streaming_mode=False)
+
+
 def _compare(out, r, frames):
     agree = 0
     while agree < frames and np.array_equal(r["codes"][agree], out.codes[0, agree]):
@@ -61,18 +67,41 @@ def test_logits_match_an_oracle_that_holds_the_same(bind, hold, shape, fmt):
 def test_contexts_of_several_parts(bind, hold, golden, fmt):
     """A reference of 600 frames in the prompt: the decode steps join parts of the key range, the prompt spans many tiles; a short
     utterance shares the batch."""
-    from qwen3_tts_rs_amd import GenerationRequest, synthetic_model
+    from qwen3_tts_rs_amd import synthetic_model
     m, cfg, _, _ = synthetic_model("T0", dtype="bf16", codec=False, round_to_bf16=True, kv_cache=fmt)
     o, _, _, _ = make_oracle(bind, "T0", "bf16", talker=True, codec=False)
     try:
         ref = np.resize(golden["ref_codes"], (600, golden["ref_codes"].shape[1]))
-        req = GenerationRequest(text_ids=golden["text_ids"], language="english", speaker_embed=golden["xvector"], ref_codes=ref,
-                                ref_text_ids=golden["ref_text_ids"], non_streaming_mode=False)
+        req = _icl_request(golden, ref)
         out = m.generate([req, _req(golden["text_ids"])], _sampling(GREEDY), 6, trace=True)
         hold(TOP[fmt])
         r = o.generate(golden["text_ids"], bind.resolve_codec_prefill(cfg, "english", None), GREEDY, 6, speaker_embed=golden["xvector"],
                        ref_text_ids=golden["ref_text_ids"], ref_codes=ref, non_streaming=False, trace=True)
         _compare(out, r, 6)
+    finally:
+        m.close()
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_sliding_window(bind, hold, golden, fmt):
+    """A talker with a window of 20 keys: prompt rows and decode steps beyond it."""
+    from conftest import SEED
+    from qwen3_tts_rs_amd import LoaderConfig, Model, round_bf16, synth
+    cfg, _, tmpl = synth.shape_set("T0")
+    cfg["talker_config"]["sliding_window"] = 20
+    m = Model(cfg, None, LoaderConfig(dtype="bf16", kv_cache=fmt))
+    m.load_weights((k, round_bf16(a)) for k, a in synth.iter_weights(synth.talker_keys(cfg), SEED))
+    m.finalize()
+    o, _, _, _ = make_oracle(bind, "T0", "bf16", talker=True, codec=False)
+    o.set_model_config(cfg)
+    try:
+        ref = np.resize(golden["ref_codes"], (90, golden["ref_codes"].shape[1]))
+        req = _icl_request(golden, ref)
+        out = m.generate([req], _sampling(GREEDY), 8, trace=True)
+        hold(TOP[fmt])
+        r = o.generate(golden["text_ids"], bind.resolve_codec_prefill(cfg, "english", None), GREEDY, 8, speaker_embed=golden["xvector"],
+                       ref_text_ids=golden["ref_text_ids"], ref_codes=ref, non_streaming=False, trace=True)
+        _compare(out, r, 8)
     finally:
         m.close()
 
