@@ -267,7 +267,8 @@ int qtts_speaker_embed_mel(qtts_model* m, const float* mel, const int* n_frames,
  * A cache holds `pages` pages of `page_tokens` tokens for each of `layers` layers.  Formats: QTTS_KV_BF16, or 8 bits in blocks of
  * 32 consecutive elements of a head row with one power-of-two scale 2^e each (1.03 bytes an element): with a = max |x| of the block,
  * e is the smallest integer >= -100 with a <= 448 * 2^e (QTTS_KV_E4M3) or a <= 127 * 2^e (QTTS_KV_INT8), and an element is held
- * as x * 2^-e rounded to nearest even (what rounds up to 2^128 reads back as infinity, as in bf16).  A block with an infinity or a NaN reads back as NaN throughout.  A new cache holds zeros.
+ * as x * 2^-e rounded to nearest even (what rounds up to 2^128 reads back as infinity, as in bf16).  A block with an infinity or a
+ * NaN reads back as NaN throughout.  A new cache holds zeros.
  *
  * Every array below is memory of the cache's GPU.  The calls enqueue kernels on `stream` (a hipStream_t of that GPU; NULL is its
  * default stream) and return; they allocate nothing, do not wait and may be captured into a graph, which reads the arrays' contents
@@ -288,7 +289,8 @@ typedef struct {
  * positions ctx_len[b]-n .. ctx_len[b]-1 of the sequence, whose position p lies on page page_table[b][p / page_tokens].  n may be 0.
  * Entries outside 0 .. pages-1 are holes: their tokens are not written, read back as zeros, and attention does not see them (pages
  * behind a sliding window can be given back).  Rows behind q_start[n_seq] are left as they are.  Pages may be shared by
- * sequences that only read them; of two tokens written to one place in one call, either's elements may remain.
+ * sequences that only read them; a place that two tokens of one call are written to holds unspecified values until it is written
+ * again (8-bit codes of one may stand beside the scale of the other).
  * The host integers bound what the device arrays hold: lengths beyond them are cut, so that no content of the arrays leads outside
  * a buffer. */
 typedef struct {
@@ -302,19 +304,20 @@ typedef struct {
     const int32_t* page_table; /* [n_seq][max_pages] */
 } qtts_kv_batch;
 /* k and v rows [n_tokens][kv_heads][head_dim] with strides in elements; the head_dim elements of a row are contiguous, pointers and
- * strides are multiples of 16 bytes. */
+ * strides (of dimensions longer than one) are multiples of 16 bytes. */
 typedef struct {
     void *k, *v;
     int dtype;                /* QTTS_F32 or QTTS_BF16 */
     int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
 } qtts_kv_rows;
-/* q and out rows [n_tokens][n_heads][head_dim], bf16; strides as above. */
+/* q and out rows [n_tokens][n_heads][head_dim], bf16; strides as above.  out may be q, with the same strides; otherwise the two do not
+ * overlap. */
 typedef struct {
     const void* q;
     void* out;
     int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
     int n_heads;              /* a multiple of kv_heads: heads h * n_heads / kv_heads .. share kv head h */
-    float scale;              /* of the scores, > 0 */
+    float scale;              /* of the scores, > 0, at most 1e30 */
     int window;               /* a token sees at most this many keys, its own included; 0 = all */
     void* workspace;          /* qtts_kv_attend_workspace bytes, 16-byte aligned; used until the call's kernels have run */
     int64_t workspace_bytes;
@@ -328,8 +331,9 @@ int qtts_kv_write(qtts_kv_cache* kv, int layer, const qtts_kv_batch* batch, cons
 /* Reads the batch's tokens back (the values they are held as); with n = ctx_len whole sequences. */
 int qtts_kv_read(qtts_kv_cache* kv, int layer, const qtts_kv_batch* batch, const qtts_kv_rows* rows, void* stream);
 /* out = softmax(scale q k^T) v of the batch's tokens over the held keys and values: a token at position p sees positions
- * p-window+1 .. p (0 .. p without a window); a row that sees nothing, or whose every score is -infinity, is zero.  The tokens' own keys and values have been
- * written before.  The workspace size depends on the batch's host integers only. */
+ * p-window+1 .. p (0 .. p without a window); a row that sees nothing, or whose every score is
+ * -infinity, is zero.  The tokens' own keys and values have been written before.  The workspace size depends on the batch's host
+ * integers only. */
 int qtts_kv_attend_workspace(qtts_kv_cache* kv, const qtts_kv_batch* batch, int n_heads, int window, int64_t* bytes);
 int qtts_kv_attend(qtts_kv_cache* kv, int layer, const qtts_kv_batch* batch, const qtts_kv_attend_args* args, void* stream);
 

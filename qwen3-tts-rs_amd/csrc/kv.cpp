@@ -3,7 +3,6 @@
 #include "generate.hpp"
 #include "kv_index.hpp"
 
-#include <cmath>
 
 namespace qtts {
 
@@ -91,6 +90,8 @@ static KvBatch check_batch(const KvCache& k, int layer, const qtts_kv_batch& b) 
 static void check_rows(const void* p, int64_t n, int64_t heads, int64_t d, int64_t ts, int64_t hs, int64_t es, bool output, const char* what) {
     const std::string name(what);
     QTTS_CHECK(p, ERR_BAD_ARG, name + ": null tensor");
+    if (n <= 1) ts = 0;  // the stride of a single token or head is not used
+    if (heads == 1) hs = 0;
     QTTS_CHECK(((uintptr_t)p & 15) == 0 && ts * es % 16 == 0 && hs * es % 16 == 0, ERR_BAD_ARG, name + ": pointer and strides must be multiples of 16 bytes");
     QTTS_CHECK(ts >= 0 && hs >= 0 && ts < (int64_t)1 << 40 && hs < (int64_t)1 << 40, ERR_BAD_ARG, name + ": stride out of range");
     if (output)
@@ -134,7 +135,7 @@ int64_t kv_attend_workspace(const KvCache& k, const qtts_kv_batch& b, int n_head
 void kv_attend(const KvCache& k, int layer, const qtts_kv_batch& b, const qtts_kv_attend_args& r, hipStream_t st) {
     KvAttendArgs a{};
     a.b = check_batch(k, layer, b);
-    QTTS_CHECK(std::isfinite(r.scale) && r.scale > 0.f, ERR_BAD_ARG, "kv attend: scale must be positive and finite");
+    QTTS_CHECK(r.scale > 0.f && r.scale <= 1e30f, ERR_BAD_ARG, "kv attend: scale must be positive and at most 1e30");
     if (b.n_seq == 0 || b.n_tokens == 0 || b.max_new == 0) {
         QTTS_CHECK(r.n_heads >= 1 && r.n_heads % k.nkv == 0, ERR_SHAPE, "kv attend: query heads must be a multiple of the cache's kv heads");
         return;

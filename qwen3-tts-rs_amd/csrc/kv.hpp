@@ -73,16 +73,16 @@ struct KvAttendArgs {
 // parts of the key range whose partial results a second launch joins.
 constexpr int KV_MAX_PARTS = 256;
 struct KvAttendPlan {
-    int tile_rows;          // 16: one wave walks keys by itself; 128: four waves share the keys through LDS
+    int tile_rows;          // 16: four waves share the rows and each walks keys of its own; 128: four waves of 32 rows share the keys through LDS
     int tiles;              // row tiles a sequence and kv head can have
     int splits, split_len;  // parts, and keys in each (a multiple of 128)
     size_t ws_bytes;
 };
 void launch_kv_attend(hipStream_t st, KvAttendArgs a, const KvAttendPlan& p);
 
-// one launch with its error as an exception (hipGetLastError would also report what other code left there)
-// The talker's cache in 8 bits (generate.cpp): rows that own consecutive pages, and the batch of the launch at hand.  The plan does not depend on what else is in the batch: single tokens in parts of KV_TALKER_PART keys, prompts in
-// tiles with all of their keys, so that a row's result is the same whatever rows it shares a launch with.
+// The talker's cache in 8 bits (generate.cpp): rows that own consecutive pages, and the batch of the launch at hand.  The plan does not
+// depend on what else is in the batch: single tokens in parts of KV_TALKER_PART keys, prompts in tiles with all of their keys, so that
+// a row's result is the same whatever rows it shares a launch with.
 constexpr int KV_TALKER_PART = 512;
 struct KvStack {
     KvLayer base{};
@@ -98,6 +98,7 @@ struct KvStack {
     }
 };
 
+// one launch with its error as an exception (hipGetLastError would also report what other code left there)
 template <typename A>
 void kv_launch(void (*kernel)(A), dim3 grid, dim3 block, hipStream_t st, A args) {
     void* p[] = {&args};

@@ -20,8 +20,9 @@ from ._lib import KV_FORMATS, QTTS_BF16, QTTS_F32, QttsError, check
 
 class KVBatch:
     """The sequences of a call (qtts_kv_batch): device int32 tensors q_start (n_seq + 1), ctx_len (n_seq) and page_table
-    (n_seq, max_pages), and the host bounds on what they hold.  A captured call reads the tensors when it is replayed, so a
-    serving loop may move the lengths on in place.  `KVCache.batch` makes one from host lists."""
+    (n_seq, max_pages), and the host bounds on what they hold (a length beyond its bound is cut).  A captured call reads the tensors
+    when it is replayed, so a serving loop may move the lengths on in place, up to max_ctx.  `KVCache.batch` makes one from host lists,
+    with bounds that just hold them."""
 
     def __init__(self, q_start, ctx_len, page_table, n_tokens: int, max_new: int, max_ctx: int):
         import torch
@@ -95,8 +96,8 @@ class KVCache:
 
     # ------------------------------------------------------------------ batches
     def batch(self, new: Sequence[int], ctx: Sequence[int], page_table) -> KVBatch:
-        """Sequence b's last new[b] of ctx[b] tokens; page_table (n_seq, max_pages): an int32 tensor on the cache's GPU, or host
-        numbers.  The rows of the calls' tensors are the sequences' new tokens one after another."""
+        """Sequence b's last new[b] of ctx[b] tokens; page_table (n_seq, max_pages): an int32 tensor on the cache's GPU (copied if it
+        is not contiguous), or host numbers.  The rows of the calls' tensors are the sequences' new tokens one after another."""
         import torch
         new, ctx = [int(x) for x in new], [int(x) for x in ctx]
         if len(new) != len(ctx) or any(n < 0 or n > c for n, c in zip(new, ctx)):
@@ -162,7 +163,7 @@ class KVCache:
     def attend(self, layer: int, batch: KVBatch, q, scale: Optional[float] = None, window: int = 0, out=None):
         """softmax(scale q k^T) v of the batch's tokens over what the cache holds for their sequences: q (n_tokens, heads, head_dim)
         bf16, heads a multiple of kv_heads; scale defaults to head_dim ** -0.5.  A token sees the positions up to its own, with a
-        window the last `window` of them.  The tokens' own keys and values have been written before."""
+        window the last `window` of them.  out: a tensor to fill, which may be q itself.  The tokens' own keys and values have been written before."""
         self._check("KVCache.attend", layer, batch, q, 0, (self._bf16,))
         heads, window = q.shape[1], min(int(window), 0x7fffffff)
         if out is None:

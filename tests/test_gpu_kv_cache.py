@@ -463,6 +463,20 @@ def test_many_sequences_and_output_over_the_queries(new):
     check_attend(pick(out, [new] * n), pick(q, [new] * n), pick(k, ctx), pick(v, ctx), [new] * len(some), [ctx[i] for i in some], "int8", d ** -0.5)
 
 
+def test_single_token_and_single_head_ignore_their_stride():
+    """The stride of a dimension of one element is not used, whatever torch says it is."""
+    d, page, ctx = 64, 16, 37
+    table, pages = table_of([ctx], page)
+    cache = KVCache(pages=pages, kv_heads=1, head_dim=d, page_tokens=page)
+    k, v, q = rand((ctx, 1, d), 1), rand((ctx, 1, d), 2), rand((1, 1, d), 3)
+    odd = lambda x: torch.as_strided(x, x.shape, (x.stride(0) if x.shape[0] > 1 else 3, 5, 1))  # noqa: E731
+    cache.write(0, cache.batch([ctx], [ctx], table), odd(k), odd(v))
+    b = cache.batch([1], [ctx], table)
+    out = torch.empty_like(q)
+    cache.attend(0, b, odd(q), out=odd(out))
+    check_attend(out, q, k, v, [1], [ctx], "bf16", d ** -0.5)
+
+
 @pytest.mark.parametrize("heads", [1, 40])
 def test_scores_that_are_not_finite(heads):
     """Overflowing scores: +infinity makes the row NaN, -infinity leaves the key without weight."""
@@ -475,7 +489,11 @@ def test_scores_that_are_not_finite(heads):
     k[3, 0, 0] = -1e38                     # -infinity for both rows
     cache.write(0, cache.batch([ctx], [ctx], table), k, v)
     b = cache.batch([2], [ctx], table)
-    check_attend(cache.attend(0, b, q), q, k[:, :, :], v, [2], [ctx], "bf16", d ** -0.5)
+    check_attend(cache.attend(0, b, q), q, k, v, [2], [ctx], "bf16", d ** -0.5)
+    k[:, 0, 0] = -1e38                     # every score -infinity: no key has weight
+    cache.write(0, cache.batch([ctx], [ctx], table), k, v)
+    assert (cache.attend(0, b, q) == 0).all()
+    k[:, 0, 0] = 0
     k[ctx - 1, 0, 0] = 1e38                # +infinity for the last row only
     cache.write(0, cache.batch([ctx], [ctx], table), k, v)
     out = cache.attend(0, b, q)
