@@ -103,17 +103,22 @@ inline KvAttendPlan kv_attend_plan(const KvLayer& kv, const KvBatch& b, int nh, 
         const long want = std::max<long>(1, 512 / std::max<long>(units, 1)), most = std::max<long>(1, (keys + 255) / 256);
         p.splits = (int)std::min<long>(std::min(want, most), KV_MAX_PARTS);
     } else {
-        // 512 blocks run at once.  Parts are worth their join where without them the last round of blocks is mostly empty: the fewest
-        // parts that fill it to nine tenths, else the best.  Measured: 384 tiles of up to 15013 e4m3 keys 508 us in one part, 400 us in four;
-        // 256 tiles of 20480 keys 564 / 404 / 420 us in 1 / 2 / 8 parts; where the rounds are full (2 x 4096 tokens, 1024 tiles) parts cost more
-        // than they give (185 us, 217 us in two).
-        double best = 0;
-        for (int s = 1; s <= KV_MAX_PARTS && best < 0.9; ++s) {
-            const long blocks = units * s;
-            if (s > 1 && keys < (blocks > 512 ? 1024L : 256L) * s) break;
-            const double fill = (double)blocks / (double)((blocks + 511) / 512 * 512);
-            if (fill > best) {
-                best = fill;
+        // The parts' number with the least time by this account: a CU walks 64 keys with one, two (three at head_dim 64) resident blocks in
+        // the microseconds below; a block costs two walks on top; parts cost a launch and their partial results, written and read at 5 TB/s.
+        // Measured with 1 / 2 / 4 / 8 parts (d = 128, bf16): 64 tiles of 8192 keys 215 119 69 58 us, 256 of them 217 178 182 205, 384 of them
+        // 296 292 292 328, 512 of them 349 370 388 438; 256 tiles of up to 512 keys 22 34 36 37; 512 of up to 4096 120 121 131 140 (the keys a
+        // tile of a prompt sees depend on its place, the account takes the most for all).
+        static constexpr float WALK[2][4] = {{0.f, 1.2f, 1.6f, 2.4f}, {0.f, 1.65f, 2.7f, 0.f}};
+        const int most = kv.d == 64 ? 3 : 2;  // resident blocks of a CU
+        const float* walk = WALK[kv.d == 64 ? 0 : 1];
+        float best = 0.f;
+        for (int s = 1; s <= KV_MAX_PARTS; ++s) {
+            const long blocks = units * s, full = blocks / (256 * most), rest = blocks % (256 * most);
+            if (s > 1 && (keys < 256L * s || blocks > 1024L * most)) break;
+            float t = (float)((keys + 64 * s - 1) / (64 * s) + 2) * ((float)full * walk[most] + walk[(rest + 255) / 256]);
+            if (s > 1) t += 4.f + (float)blocks * (float)(p.tile_rows * kv.d * 8) / 5e6f;
+            if (s == 1 || t < best) {
+                best = t;
                 p.splits = s;
             }
         }
