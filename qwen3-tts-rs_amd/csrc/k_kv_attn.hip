@@ -457,17 +457,20 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kt][i] * sc);
-        mx = fold_halves(mx, fmax2);
-        const float mn = fmaxf(m, mx);
-        const float ref = mn == -INFINITY ? 0.f : mn;
-        if (__any(mn > m)) {
-            const float alpha = __builtin_amdgcn_exp2f(m - ref);
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kt][i]);
+        mx = fold_halves(mx, fmax2) * sc;
+        // The reference m of the exponentials need not be the maximum, only near it: it moves when a row's maximum has left it by more than
+        // 2^8 (p and l stay far from overflow, their relative precision is the same).  Moved at every new maximum, which some row of 32 has in
+        // most blocks, acc's scaling was a fifth of the vector instructions.
+        if (__any(mx > m + 8.f)) {
+            const float mn = fmaxf(m, mx);
+            const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
             l *= alpha;
 #pragma unroll
             for (int dt = 0; dt < NDT; ++dt) acc[dt] *= alpha;
             m = mn;
         }
+        const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
