@@ -323,6 +323,7 @@ typedef struct {
     int64_t workspace_bytes;
 } qtts_kv_attend_args;
 int qtts_kv_open(qtts_ctx* ctx, const qtts_kv_config* cfg, qtts_kv_cache** out);
+/* Waits for the GPU to finish with the memory.  Before qtts_shutdown of the cache's context. */
 void qtts_kv_close(qtts_kv_cache* kv);
 /* Device memory of the cache. */
 int64_t qtts_kv_bytes(qtts_kv_cache* kv);

@@ -1,6 +1,7 @@
 // Writing keys and values into the paged cache and reading them back (gfx950), and the talker's projection pass that ends in it.
 //
-// Both directions are bound by the bytes they move; nothing is reused.  Writing, a lane owns 16 elements: loads may come in pieces (a
+// Both directions are bound by the bytes they move; nothing is reused.  16 x 8192 tokens of 8 heads (d = 128) between bf16 tensors and int8 pages:
+// written in 145 us (4.3 TB/s read + written), read back in 130 us (4.8; a large copy reaches 4.89).  Writing, a lane owns 16 elements: loads may come in pieces (a
 // line's other pieces are in the cache by then), stores should not, and 16 codes leave as 16 bytes; two neighbouring lanes hold a
 // block of 32 and share its largest element with one lane swap.  Reading back, a lane owns 16 bytes of the caller's row, so that a
 // wave's store is contiguous (84 MB of f32: 26 us with 64-byte pieces per lane, 16 us so).  A thread has two or four rows in flight;
@@ -161,7 +162,7 @@ void launch_kv_read(hipStream_t st, int dtype, const KvMoveArgs& a) { launch_kv_
 
 // Split-K combine, bias, per-head RMSNorm and RoPE as in qkv_post_kernel (k_attn.hip), one wave per (token, head); a lane holds
 // the rotation pair (i, i + d / 2), so a block of 32 elements lies in 32 neighbouring lanes and its largest element is a reduction
-// over half a wave.
+// over half a wave.  Latency, not bytes: 64 tokens of 16 + 2 x 8 heads take 4.8 us (as the same pass over a bf16 cache does), 3264 prompt tokens 31 us.
 struct KvPostArgs {
     QkvPostArgs p;
     KvLayer kv;

@@ -11,7 +11,7 @@
 //                 which the lanes hold them; V^T comes out of a row-major LDS image by transposing reads.
 // Rounding: K, V and Q enter exactly (bf16, or codes times a power of two).  P is rounded to bf16 for the second product, at most
 // 2^-8 relative per term, as the output itself is afterwards; l is summed from the unrounded f32 values.
-// Key ranges of few rows are cut into parts (KvAttendPlan) whose (m, l, O) a second launch joins.
+// Key ranges are cut into parts where a call has too few tiles to fill the GPU (kv_attend_plan); a second launch joins their (m, l, O).
 // A masked key may hold anything: its score is replaced, and its V row meets the products as zero.  Where some rows of a tile see a key
 // and others do not, a non-finite V element is taken out of the products and added to the rows that see it one by one.
 #include "kv_device.hpp"
@@ -52,10 +52,17 @@ __device__ __forceinline__ u32x4_t keep(u32x4_t w, bool in) { return in ? w : u3
 // value added to a row that sees a V element: the element if it is not finite (it was taken out of the products), else nothing
 __device__ __forceinline__ float bad_only(u16 b) { return (b & 0x7f80u) == 0x7f80u ? bf16_bits_to_f32(b) : 0.f; }
 
-// ---------------------------------------------------------------------------------------------- at most 16 rows a tile
-template <int FMT, int D>
-__global__ __launch_bounds__(256, 3) void kv_attend_few_kernel(KvAttendArgs a) {
+// ---------------------------------------------------------------------------------------------- 16 or 32 rows a tile
+// Single tokens and drafts: bound by the bytes of the cache, so keys go from the cache into registers in operand order (a lane's 16 bytes
+// of a K row are its share of the A operand), only V passes through LDS for its transpose, and no wave waits for another before the end:
+// each walks every fourth group of 32 keys with the next group's loads in flight, and the four results are joined in LDS.  32 rows share
+// one walk (and one conversion of 8-bit keys) instead of walking twice.  Measured (d = 128): 12 x 30011 int8 keys of 8 kv heads 124 us with the join = 4.8 TB/s
+// (a large copy: 4.89), 64 x 500 e4m3 keys 13 us = 3.9 TB/s, 32 x 2047 int8 keys with five tokens 27 us (+ 5 us of joining), 113 keys of one sequence 6 us,
+// of which all is latency.  Four waves a SIMD instead of three spilled registers and were slower.
+template <int FMT, int D, int RG>
+__global__ __launch_bounds__(256, RG == 1 ? 3 : 2) void kv_attend_few_kernel(KvAttendArgs a) {
     constexpr bool Q8 = FMT != KV_BF16;
+    constexpr int TR = 16 * RG;                        // a lane holds scores of RG rows, 16 apart
     constexpr int NJ = D / 32, NDT = D / 16;
     constexpr int KLD = Q8 ? D / 64 : D / 32;          // 16-byte loads of a K row per lane
     constexpr int EPP = Q8 ? 16 : 8, PPR = D / EPP;    // V: elements per 16-byte piece, pieces per row
@@ -64,36 +71,44 @@ __global__ __launch_bounds__(256, 3) void kv_attend_few_kernel(KvAttendArgs a) {
     constexpr int LDO = D + 4;
     constexpr int VBYTES = 4 * 32 * LDV * 2, OBYTES = 4 * 16 * LDO * 4;
     __shared__ __attribute__((aligned(16))) unsigned char smem[VBYTES > OBYTES ? VBYTES : OBYTES];
-    __shared__ float pm[4][16], pl[4][16];
+    __shared__ float pm[4][TR], pl[4][TR];
 
     const int pair = blockIdx.x;
     if (pair >= a.b.n_seq * a.kv.nkv) return;
-    const KvTile t = kv_tile<16>(a, pair, blockIdx.y, blockIdx.z);
+    const KvTile t = kv_tile<TR>(a, pair, blockIdx.y, blockIdx.z);
     if (!t.live) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, gq = lane >> 4;
     u16* Vs = reinterpret_cast<u16*>(smem) + wave * 32 * LDV;
 
-    // this lane's row: its key range and its query
-    const int row = t.row0 + r;
-    const bool has = row < t.rows;
-    const int tok = (has ? row : t.row0) / t.G, head = t.g * t.G + (has ? row : t.row0) - tok * t.G;
-    const int pos = t.s.ctx - t.s.n + tok;
-    const int klo = has ? (a.window ? pos - a.window + 1 : 0) : 0x7fffffff;
-    bf16x8_t q[NJ];
-    {
+    // this lane's rows: their key ranges and queries
+    int pos[RG], klo[RG];
+    bool has[RG];
+    bf16x8_t q[RG][NJ];
+#pragma unroll
+    for (int rg = 0; rg < RG; ++rg) {
+        const int row = t.row0 + 16 * rg + r;
+        has[rg] = row < t.rows;
+        const int rr = has[rg] ? row : t.row0, tok = rr / t.G, head = t.g * t.G + rr - tok * t.G;
+        pos[rg] = t.s.ctx - t.s.n + tok;
+        klo[rg] = has[rg] ? (a.window ? pos[rg] - a.window + 1 : 0) : 0x7fffffff;
         const u16* qp = (const u16*)a.q + (long)(t.s.t0 + tok) * a.q_token_stride + (long)head * a.q_head_stride;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             const int d0 = Q8 ? 64 * (j >> 1) + 16 * gq + 8 * (j & 1) : 32 * j + 8 * gq;
-            q[j] = *reinterpret_cast<const bf16x8_t*>(qp + d0);
+            q[rg][j] = *reinterpret_cast<const bf16x8_t*>(qp + d0);
         }
     }
 
-    f32x4_t acc[NDT];
+    f32x4_t acc[RG][NDT];
+    float m[RG], l[RG];
 #pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) acc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
+    for (int rg = 0; rg < RG; ++rg) {
+        m[rg] = -INFINITY;
+        l[rg] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) acc[rg][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
     const float sc = a.scale * 1.4426950408889634f;  // exponentials to base 2
 
     u32x4_t kreg[2][KLD], vreg[NV];
@@ -164,23 +179,30 @@ __global__ __launch_bounds__(256, 3) void kv_attend_few_kernel(KvAttendArgs a) {
             for (int h = 0; h < (Q8 ? 2 : 1); ++h)
                 *reinterpret_cast<u32x4_t*>(Vs + (n * RPI + lane / PPR) * LDV + (lane % PPR) * EPP + 8 * h) = w[h];
         }
-        // scores of 2 x 16 keys: s[kt][i] = key kb + 16 kt + 4 gq + i
-        f32x4_t s[2];
+        // scores of 2 x 16 keys: s[rg][kt][i] = key kb + 16 kt + 4 gq + i
+        f32x4_t s[RG][2];
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
-            s[kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int rg = 0; rg < RG; ++rg) s[rg][kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
             if constexpr (Q8) {
 #pragma unroll
                 for (int j = 0; j < KLD; ++j) {
                     const float f = kv_scale((ksc[kt] >> (8 * (2 * j + (gq >> 1)))) & 0xffu);
                     const u32x4_t c = kreg[kt][j];
-                    s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kv_decode8<FMT>(c.x, c.y, f)), q[2 * j], s[kt], 0, 0, 0);
-                    s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kv_decode8<FMT>(c.z, c.w, f)), q[2 * j + 1], s[kt], 0, 0, 0);
+                    const bf16x8_t k0 = __builtin_bit_cast(bf16x8_t, kv_decode8<FMT>(c.x, c.y, f)), k1 = __builtin_bit_cast(bf16x8_t, kv_decode8<FMT>(c.z, c.w, f));
+#pragma unroll
+                    for (int rg = 0; rg < RG; ++rg) {
+                        s[rg][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, q[rg][2 * j], s[rg][kt], 0, 0, 0);
+                        s[rg][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, q[rg][2 * j + 1], s[rg][kt], 0, 0, 0);
+                    }
                 }
             } else {
 #pragma unroll
                 for (int j = 0; j < KLD; ++j)
-                    s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kreg[kt][j]), q[j], s[kt], 0, 0, 0);
+#pragma unroll
+                    for (int rg = 0; rg < RG; ++rg)
+                        s[rg][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kreg[kt][j]), q[rg][j], s[rg][kt], 0, 0, 0);
             }
         }
         // the next rows travel while these go through the softmax
@@ -189,38 +211,44 @@ __global__ __launch_bounds__(256, 3) void kv_attend_few_kernel(KvAttendArgs a) {
         load(kb + 128, pg);  // behind the part: page 0, not used
         pv = kv_page16(a, t, kb + 256 + 16 * (lane & 1));
 
-        float p[8], mx = -INFINITY;
+        bf16x8_t ph[RG];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int key = kb + 16 * (e >> 2) + 4 * gq + (e & 3);
-            const bool see = key >= klo && key <= pos && key < t.s1 && pc[e >> 2] >= 0;
-            p[e] = see ? s[e >> 2][e & 3] * sc : -INFINITY;
-            mx = fmaxf(mx, p[e]);
+        for (int rg = 0; rg < RG; ++rg) {
+            float p[8], mx = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int key = kb + 16 * (e >> 2) + 4 * gq + (e & 3);
+                const bool see = key >= klo[rg] && key <= pos[rg] && key < t.s1 && pc[e >> 2] >= 0;
+                p[e] = see ? s[rg][e >> 2][e & 3] * sc : -INFINITY;
+                mx = fmaxf(mx, p[e]);
+            }
+            const float mn = fmaxf(m[rg], kv_quad_rows(mx, fmax2));
+            const float ref = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: every exponential below is 0
+            const float alpha = __builtin_amdgcn_exp2f(m[rg] - ref);
+            m[rg] = mn;
+            float ps = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                p[e] = __builtin_amdgcn_exp2f(p[e] - ref);
+                ps += p[e];
+            }
+            l[rg] = l[rg] * alpha + ps;
+            ph[rg] = __builtin_bit_cast(bf16x8_t, u32x4_t{pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]), pack_bf16(p[4], p[5]), pack_bf16(p[6], p[7])});
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) acc[rg][dt] *= alpha;
         }
-        const float mn = fmaxf(m, kv_quad_rows(mx, fmax2));
-        const float ref = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: every exponential below is 0
-        const float alpha = __builtin_amdgcn_exp2f(m - ref);
-        m = mn;
-        float ps = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            p[e] = __builtin_amdgcn_exp2f(p[e] - ref);
-            ps += p[e];
-        }
-        l = l * alpha + ps;
-        const bf16x8_t ph = __builtin_bit_cast(bf16x8_t, u32x4_t{pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]), pack_bf16(p[4], p[5]), pack_bf16(p[6], p[7])});
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) acc[dt] *= alpha;
         __builtin_amdgcn_wave_barrier();  // the image is this wave's own: its LDS accesses are served in order
         if (mixed && __any(bad)) {
             for (int j = 0; j < 32; ++j) {
                 const int key = kb + j;
-                if (key >= klo && key <= pos && has) {
 #pragma unroll
-                    for (int dt = 0; dt < NDT; ++dt)
+                for (int rg = 0; rg < RG; ++rg)
+                    if (key >= klo[rg] && key <= pos[rg] && has[rg]) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[dt][i] += bad_only(Vs[j * LDV + 16 * dt + 4 * gq + i]);
-                }
+                        for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) acc[rg][dt][i] += bad_only(Vs[j * LDV + 16 * dt + 4 * gq + i]);
+                    }
             }
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -236,62 +264,75 @@ __global__ __launch_bounds__(256, 3) void kv_attend_few_kernel(KvAttendArgs a) {
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) {
             const bf16x8_t vt = join8(read_tr4(vrow + 16 * dt), read_tr4(vrow + 16 * LDV + 16 * dt));
-            acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt, ph, acc[dt], 0, 0, 0);
+#pragma unroll
+            for (int rg = 0; rg < RG; ++rg) acc[rg][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt, ph[rg], acc[rg][dt], 0, 0, 0);
         }
         __builtin_amdgcn_wave_barrier();
     }
 
-    // join the four waves
-    l = kv_quad_rows(l, fadd2);
-    __syncthreads();
+    // join the four waves, 16 rows at a time
     float* Os = reinterpret_cast<float*>(smem);
-    if (gq == 0) {
-        pm[wave][r] = m;
-        pl[wave][r] = l;
-    }
-#pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) *reinterpret_cast<f32x4_t*>(Os + (wave * 16 + r) * LDO + 16 * dt + 4 * gq) = acc[dt];
-    __syncthreads();
     constexpr int EPT = D / 16;
     const int orow = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * EPT;
-    if (t.row0 + orow >= t.rows) return;
-    float M = pm[0][orow];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) M = fmaxf(M, pm[w][orow]);
-    float L = 0.f, o[EPT];
-#pragma unroll
-    for (int e = 0; e < EPT; ++e) o[e] = 0.f;
-    const float ref = M == -INFINITY ? 0.f : M;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        const float wt = __builtin_amdgcn_exp2f(pm[w][orow] - ref);
-        L += wt * pl[w][orow];
-#pragma unroll
-        for (int e = 0; e < EPT; ++e) o[e] += wt * Os[(w * 16 + orow) * LDO + d0 + e];
-    }
-    if (t.parts > 1) {
-        const size_t u = ((size_t)(pair * a.tiles + blockIdx.y) * a.splits + blockIdx.z) * 16 + orow;  // slot
-        float* po = a.ws + u * D + d0;
-#pragma unroll
-        for (int e = 0; e < EPT; e += 4) *reinterpret_cast<float4*>(po + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-        if ((threadIdx.x & 15) == 0) {
-            float* ml = a.ws + (size_t)a.b.n_seq * a.kv.nkv * a.tiles * a.splits * 16 * D + u * 2;
-            ml[0] = M;
-            ml[1] = L;
+    for (int rg = 0; rg < RG; ++rg) {
+        const float lr = kv_quad_rows(l[rg], fadd2);
+        __syncthreads();
+        if (gq == 0) {
+            pm[wave][16 * rg + r] = m[rg];
+            pl[wave][16 * rg + r] = lr;
         }
-        return;
-    }
-    const int rr = t.row0 + orow, tk = rr / t.G, hd = t.g * t.G + rr - tk * t.G;
-    bf16_t* op = (bf16_t*)a.out + (long)(t.s.t0 + tk) * a.out_token_stride + (long)hd * a.out_head_stride + d0;
-    const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
-    for (int e = 0; e < EPT; e += 4) {
-        const float v[4] = {o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv};
-        store4_split(op + e, a.out_lo, v);
+        for (int dt = 0; dt < NDT; ++dt) *reinterpret_cast<f32x4_t*>(Os + (wave * 16 + r) * LDO + 16 * dt + 4 * gq) = acc[rg][dt];
+        __syncthreads();
+        const int trow = 16 * rg + orow, rr = t.row0 + trow;
+        if (rr >= t.rows) continue;
+        float M = pm[0][trow];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) M = fmaxf(M, pm[w][trow]);
+        float L = 0.f, o[EPT];
+#pragma unroll
+        for (int e = 0; e < EPT; ++e) o[e] = 0.f;
+        const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float wt = __builtin_amdgcn_exp2f(pm[w][trow] - ref);
+            L += wt * pl[w][trow];
+#pragma unroll
+            for (int e = 0; e < EPT; ++e) o[e] += wt * Os[(w * 16 + orow) * LDO + d0 + e];
+        }
+        if (t.parts > 1) {
+            const size_t u = ((size_t)(pair * a.tiles + blockIdx.y) * a.splits + blockIdx.z) * TR + trow;  // slot
+            float* po = a.ws + u * D + d0;
+#pragma unroll
+            for (int e = 0; e < EPT; e += 4) *reinterpret_cast<float4*>(po + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            if ((threadIdx.x & 15) == 0) {
+                float* ml = a.ws + (size_t)a.b.n_seq * a.kv.nkv * a.tiles * a.splits * TR * D + u * 2;
+                ml[0] = M;
+                ml[1] = L;
+            }
+            continue;
+        }
+        const int tk = rr / t.G, hd = t.g * t.G + rr - tk * t.G;
+        bf16_t* op = (bf16_t*)a.out + (long)(t.s.t0 + tk) * a.out_token_stride + (long)hd * a.out_head_stride + d0;
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+        for (int e = 0; e < EPT; e += 4) {
+            const float v[4] = {o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv};
+            store4_split(op + e, a.out_lo, v);
+        }
     }
 }
 
 // ------------------------------------------------------------------------------------------------------ 128 rows a tile
+// Prompts and chunks: bound by the matrix and vector instructions, so 128 rows share one staging (and conversion) of 64 keys: four waves of 32
+// rows, the K and V images in LDS, the next block of keys travelling in registers, two blocks of threads a CU (three at d = 64) that fill each
+// other's waits.  Measured (d = 128): equal tiles, 1024 of them, 870 TFLOP/s in bf16, 930 in e4m3 (half the bytes from L2); a large library product
+// 1257.  Prompts of 4096 and 2912 tokens 160 us = 650 TFLOP/s: the longest tile walks 64 blocks of keys at 2.5 us; 509 new tokens behind 3 x 15013
+// e4m3 keys 380 us = 765.  Counters of the prompts: matrix pipe busy 35 % of the CUs' time, vector pipe 37 %, LDS 26 % without a
+// conflict: neither is full, a wave's chain S -> softmax -> P V is what waits.  Tried, not faster: S of the next block issued before the softmax of
+// this one over double images; 256 rows with eight waves (prompts 7 % faster, chunks and windows slower); longest tiles at a higher wave
+// priority; blocks of keys dealt evenly to the CUs (the tiles of a head no longer walk in step and miss the L2).
 template <int FMT, int D>
 __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) {
     constexpr bool Q8 = FMT != KV_BF16;
@@ -520,9 +561,9 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
 // One wave per row: its lanes take the parts' maxima and sums (64 at a time) and turn them into weights; then each lane adds up its
 // D / 64 columns of the parts' outputs with eight loads in flight: 5 us for 73 parts of 56 rows, where one thread an element and all parts in a
 // row of loads took 19 us and the kernel below takes 11 us.
-template <int D>
+template <int D, int TR>
 __global__ __launch_bounds__(256) void kv_attend_join_few_kernel(KvAttendArgs a) {
-    constexpr int TR = 16, EPL = D / 64;
+    constexpr int EPL = D / 64;
     typedef float vec_t __attribute__((ext_vector_type(EPL)));
     const int unit = blockIdx.x, pair = unit / a.tiles, tile = unit - pair * a.tiles;
     const KvTile t = kv_tile<TR>(a, pair, tile, 0);
@@ -622,17 +663,20 @@ void launch_kv_attend(hipStream_t st, KvAttendArgs a, const KvAttendPlan& p) {
     const unsigned pairs = (unsigned)(a.b.n_seq * a.kv.nkv);
     // pairs vary fastest and are padded to the number of XCDs: all tiles and parts of a pair run on one XCD and share its L2
     const dim3 grid((pairs + 7) / 8 * 8, (unsigned)p.tiles, (unsigned)p.splits);
-    const dim3 join(pairs * (unsigned)p.tiles, p.tile_rows == 16 ? 4u : (unsigned)a.kv.d / 8u);
-#define QTTS_KV_ATTEND(FMT, DD)                                                                          \
-    if (a.kv.format == FMT && a.kv.d == DD) {                                                            \
-        if (p.tile_rows == 16) {                                                                         \
-            kv_launch(kv_attend_few_kernel<FMT, DD>, grid, dim3(256), st, a);                            \
-            if (p.splits > 1) kv_launch(kv_attend_join_few_kernel<DD>, join, dim3(256), st, a);          \
-        } else {                                                                                         \
-            kv_launch(kv_attend_tile_kernel<FMT, DD>, grid, dim3(256), st, a);                           \
-            if (p.splits > 1) kv_launch(kv_attend_join_tile_kernel<DD>, join, dim3(256), st, a);         \
-        }                                                                                                \
-        return;                                                                                          \
+    const dim3 join(pairs * (unsigned)p.tiles, p.tile_rows == 128 ? (unsigned)a.kv.d / 8u : (unsigned)p.tile_rows / 4u);
+#define QTTS_KV_ATTEND(FMT, DD)                                                                         \
+    if (a.kv.format == FMT && a.kv.d == DD) {                                                           \
+        if (p.tile_rows == 16) {                                                                        \
+            kv_launch(kv_attend_few_kernel<FMT, DD, 1>, grid, dim3(256), st, a);                        \
+            if (p.splits > 1) kv_launch(kv_attend_join_few_kernel<DD, 16>, join, dim3(256), st, a);     \
+        } else if (p.tile_rows == 32) {                                                                 \
+            kv_launch(kv_attend_few_kernel<FMT, DD, 2>, grid, dim3(256), st, a);                        \
+            if (p.splits > 1) kv_launch(kv_attend_join_few_kernel<DD, 32>, join, dim3(256), st, a);     \
+        } else {                                                                                        \
+            kv_launch(kv_attend_tile_kernel<FMT, DD>, grid, dim3(256), st, a);                          \
+            if (p.splits > 1) kv_launch(kv_attend_join_tile_kernel<DD>, join, dim3(256), st, a);        \
+        }                                                                                               \
+        return;                                                                                         \
     }
     QTTS_KV_ATTEND(KV_BF16, 64)
     QTTS_KV_ATTEND(KV_E4M3, 64)

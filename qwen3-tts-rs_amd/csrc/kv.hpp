@@ -73,7 +73,7 @@ struct KvAttendArgs {
 // parts of the key range whose partial results a second launch joins.
 constexpr int KV_MAX_PARTS = 256;
 struct KvAttendPlan {
-    int tile_rows;          // 16: four waves share the rows and each walks keys of its own; 128: four waves of 32 rows share the keys through LDS
+    int tile_rows;          // 16 or 32: four waves share the rows, each walks keys of its own; 128: four waves of 32 rows share the keys through LDS
     int tiles;              // row tiles a sequence and kv head can have
     int splits, split_len;  // parts, and keys in each (a multiple of 128)
     size_t ws_bytes;

@@ -86,17 +86,17 @@ QTTS_KV_HD int kv_page16(const KvAttendArgs& a, const KvTile& t, int key) {
 inline KvAttendPlan kv_attend_plan(const KvLayer& kv, const KvBatch& b, int nh, int window) {
     KvAttendPlan p{};
     const long rows = (long)b.max_new * (nh / kv.nkv);
-    // Several 16-row tiles read their keys once each, a 128-row tile is slow to start and partly empty.  Measured with 20 / 32 / 48 / 64 rows, 16-row
-    // against 128-row tiles: 8 x 8192 bf16 keys 62 61 107 99 against 52 53 55 57 us, int8 51 51 86 88 against 50 50 57 58; 64 x 500 int8 29 30 39 49
-    // against 25 26 30 30; 2 kv heads of 8 x 2000 bf16 13 13 17 18 against 18 17 18 19.
-    p.tile_rows = rows <= 32 ? 16 : 128;
+    // Every tile walks, and in 8 bits converts, its keys by itself; a 128-row tile is slow to start and partly empty.  Measured in us (d = 128) with
+    // tiles of 16 / 32 / 128 rows: 16 rows of 128 x 8192 int8 keys 53 61 79, bf16 107 107 103, of 512 x 2000 int8 47 56 75, of 8 x 300 bf16
+    // 12 13 13; 20 rows 87 64 79, 130 114 108, 103 59 75, 12 13 13; 48 rows 152 116 91, 260 133 111, 140 107 86, 12 14 14.
+    p.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 128;
     p.tiles = (int)std::min<long>((rows + p.tile_rows - 1) / p.tile_rows, 65536);  // the grid's y: callers refuse more than 65535
     // keys the tile with the most of them can see
     const long span_tokens = std::min<long>(b.max_new, (p.tile_rows - 1) / (nh / kv.nkv) + 2);
     const long keys = std::max<long>(1, window ? std::min<long>(b.max_ctx, window + span_tokens + 63) : b.max_ctx);
     const long units = (long)b.n_seq * kv.nkv * p.tiles;
     p.splits = 1;
-    if (p.tile_rows == 16) {
+    if (p.tile_rows != 128) {
         // Two blocks a CU fill it, and a part of fewer than 256 keys is mostly start and join.  Measured with targets of 512 / 768 / 1024
         // blocks: 12 x 30011 int8 keys 124 / 131 / 140 us, 32 x 2047 with five tokens 32.2 / 30.6 / 34.0 us, 7 x 20011 bf16 keys 23.2 / 26.4 /
         // 26.5 us; parts of at least 512 keys: 24.8 us for the last.
@@ -105,8 +105,8 @@ inline KvAttendPlan kv_attend_plan(const KvLayer& kv, const KvBatch& b, int nh, 
     } else {
         // The parts' number with the least time by this account: a CU walks 64 keys with one, two (three at head_dim 64) resident blocks in
         // the microseconds below; a block costs two walks on top; parts cost a launch and their partial results, written and read at 5 TB/s.
-        // Measured with 1 / 2 / 4 / 8 parts (d = 128, bf16): 64 tiles of 8192 keys 215 119 69 58 us, 256 of them 217 178 182 205, 384 of them
-        // 296 292 292 328, 512 of them 349 370 388 438; 256 tiles of up to 512 keys 22 34 36 37; 512 of up to 4096 120 121 131 140 (the keys a
+        // Measured with 1 / 2 / 4 / 8 parts (d = 128, bf16): 64 tiles of 8192 keys 198 111 64 56 us, 256 of them 202 176 180 200, 384 of them
+        // 285 282 283 313, 512 of them 335 354 371 421; 256 tiles of up to 512 keys 21 33 36 36; 512 of up to 4096 114 113 124 134 (the keys a
         // tile of a prompt sees depend on its place, the account takes the most for all).
         static constexpr float WALK[2][4] = {{0.f, 1.2f, 1.6f, 2.4f}, {0.f, 1.65f, 2.7f, 0.f}};
         const int most = kv.d == 64 ? 3 : 2;  // resident blocks of a CU

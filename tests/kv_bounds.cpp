@@ -64,11 +64,11 @@ int main() {
         a.splits = p.splits;
         a.split_len = p.split_len;
         NEED(p.split_len % 128 == 0 && p.splits >= 1 && (p.splits == 1 || p.ws_bytes >= (size_t)n * a.kv.nkv * p.tiles * p.splits * p.tile_rows * 66 * 4));
-        if (p.tile_rows == 16 ? tiles<16>(a, trial) : tiles<128>(a, trial)) return 1;
+        if (p.tile_rows == 16 ? tiles<16>(a, trial) : p.tile_rows == 32 ? tiles<32>(a, trial) : tiles<128>(a, trial)) return 1;
         // more parts than this small range would get
         a.splits = in(1, 4);
         a.split_len = ((a.b.max_ctx + a.window + 200) / a.splits + 127) / 128 * 128 + 128;
-        if (p.tile_rows == 16 ? tiles<16>(a, trial) : tiles<128>(a, trial)) return 1;
+        if (p.tile_rows == 16 ? tiles<16>(a, trial) : p.tile_rows == 32 ? tiles<32>(a, trial) : tiles<128>(a, trial)) return 1;
         for (int s = 0; s < n; ++s) {
             const KvSeq q = kv_seq(a.b, s);
             NEED(q.t0 >= 0 && q.n >= 0 && q.n <= a.b.max_new && q.t0 + q.n <= a.b.n_tokens && q.ctx >= 0 && q.ctx <= a.b.max_ctx);

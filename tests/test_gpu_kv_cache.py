@@ -477,6 +477,38 @@ def test_single_token_and_single_head_ignore_their_stride():
     check_attend(out, q, k, v, [1], [ctx], "bf16", d ** -0.5)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("group,new", [(1, 17), (17, 1), (3, 7), (5, 5), (8, 4), (32, 1), (4, 8), (11, 3)])
+def test_17_to_33_rows(group, new, fmt, dim):
+    """Rows a kv head from just over 16 to just over 32: alone and with the keys in parts, with holes, with a window, an infinity in V that
+    some rows see."""
+    page, kv = 32, 2
+    ctx, news = [1100, new, 333], [new, new, max(1, new - 1)]
+    table, pages = table_of(ctx, page)
+    cache = KVCache(pages=pages, kv_heads=kv, head_dim=dim, format=fmt, page_tokens=page)
+    k, v, q = rand((sum(ctx), kv, dim), 1), rand((sum(ctx), kv, dim), 2), rand((sum(news), group * kv, dim), 3)
+    cache.write(0, cache.batch(ctx, ctx, table), k, v)
+    b = cache.batch(news, ctx, table)
+    assert workspace(cache, b, group * kv) > 0
+    check_attend(cache.attend(0, b, q), q, k, v, news, ctx, fmt, dim ** -0.5)
+    check_attend(cache.attend(0, b, q, window=40), q, k, v, news, ctx, fmt, dim ** -0.5, 40)
+    short = cache.batch([new], [new], table[1:2].contiguous())  # one part
+    assert workspace(cache, short, group * kv) == 0
+    sl = slice(ctx[0], ctx[0] + new)
+    q1 = q[news[0]:news[0] + new].contiguous()
+    check_attend(cache.attend(0, short, q1), q1, k[sl], v[sl], [new], [new], fmt, dim ** -0.5)
+    if new > 2:  # the last token's value: only its own rows see it
+        v[ctx[0] + new - 1, 0, 5] = float("inf")
+        cache.write(0, cache.batch([1], [new], table[1:2].contiguous()), k[sl][-1:], v[sl][-1:])
+        out = cache.attend(0, short, q1)
+        assert out[:-1].isfinite().all() and not out[-1, :group].isfinite().all() and out[-1, group:].isfinite().all()
+    table[0, 3], table[0, 30], table[2, 0] = -1, pages, -7
+    holes = [set(range(96, 128)) | set(range(960, 992)), set(), set(range(32))]
+    if new <= 2:
+        check_attend(cache.attend(0, cache.batch(news, ctx, table), q), q, k, v, news, ctx, fmt, dim ** -0.5, 0, holes)
+
+
 @pytest.mark.parametrize("heads", [1, 40])
 def test_scores_that_are_not_finite(heads):
     """Overflowing scores: +infinity makes the row NaN, -infinity leaves the key without weight."""
