@@ -192,6 +192,12 @@ impl HipModel {
         Ok(ses)
     }
 
+    /// The talker's key/value cache from the next generate call on: `sys::QTTS_KV_E4M3` or `sys::QTTS_KV_INT8` (half the memory, bf16 models),
+    /// `sys::QTTS_KV_BF16` for the model's dtype.  Sessions opened later start with the model's choice.
+    pub fn set_kv_cache(&mut self, format: i32) -> Result<(), HipError> {
+        check(unsafe { sys::qtts_model_set_kv_cache(self.m, format) })
+    }
+
     /// `ConditionalGeneration::generate` for a batch (`generate_custom_voice_from_texts_batch` makes one call of it).
     pub fn generate(&mut self, reqs: &[HipRequest], sampling: HipSampling, max_new_tokens: usize) -> Result<Vec<HipCodes>, HipError> {
         let langs: Vec<CString> = reqs.iter().map(|r| CString::new(r.language.as_str()).unwrap()).collect();

@@ -107,6 +107,7 @@ static void kv_move(const KvCache& k, int layer, const qtts_kv_batch& b, const q
     const int64_t es = (int64_t)dtype_size(r.dtype);
     check_rows(r.k, b.n_tokens, k.nkv, k.d, r.k_token_stride, r.k_head_stride, es, !write, "kv cache: k");
     check_rows(r.v, b.n_tokens, k.nkv, k.d, r.v_token_stride, r.v_head_stride, es, !write, "kv cache: v");
+    QTTS_CHECK(write || r.k != r.v, ERR_BAD_ARG, "kv cache: k and v are read into one tensor");
     a.kv = k.layer(layer, b);
     a.k_in = r.k; a.v_in = r.v; a.k_out = r.k; a.v_out = r.v;
     a.k_token_stride = r.k_token_stride; a.k_head_stride = r.k_head_stride;

@@ -165,7 +165,7 @@ class KVCache:
         bf16, heads a multiple of kv_heads; scale defaults to head_dim ** -0.5.  A token sees the positions up to its own, with a
         window the last `window` of them.  out: a tensor to fill, which may be q itself.  The tokens' own keys and values have been written before."""
         self._check("KVCache.attend", layer, batch, q, 0, (self._bf16,))
-        heads, window = q.shape[1], min(int(window), 0x7fffffff)
+        heads, window = q.shape[1], max(-1, min(int(window), 0x7fffffff))
         if out is None:
             out = self._torch.empty_like(q, memory_format=self._torch.contiguous_format)
         else:

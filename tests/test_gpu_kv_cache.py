@@ -584,6 +584,11 @@ def test_refusals():
     far = KVBatch(b.q_start, b.ctx_len, table, 2, 2, 33)  # max_ctx beyond the table's columns
     with pytest.raises(QttsError, match="max_pages"):
         cache.attend(0, far, ok)
+    with pytest.raises(QttsError, match="one tensor"):
+        cache.read(0, b, out=(ok, ok))
+    for kw in (dict(scale=1e31), dict(scale=math.inf), dict(window=-(1 << 40))):
+        with pytest.raises(QttsError):
+            cache.attend(0, b, ok, **kw)
     # a workspace that is too small
     long = KVCache(pages=64, kv_heads=1, head_dim=d, page_tokens=64)
     lb = long.batch([1], [4000], torch.arange(64, dtype=torch.int32, device="cuda").view(1, 64))
