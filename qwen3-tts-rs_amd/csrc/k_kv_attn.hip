@@ -477,11 +477,35 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[kt][i] = 0.f;
         const u16* kp = Ks + r * LDK + 8 * hf;
+        constexpr int AHEAD = 3;
+        bf16x8_t kf[AHEAD][2];
+        auto read_k = [&](int j) {
 #pragma unroll
-        for (int j = 0; j < NS; ++j)
+            for (int kt = 0; kt < 2; ++kt) kf[j % AHEAD][kt] = *reinterpret_cast<const bf16x8_t*>(kp + kt * 32 * LDK + 16 * j);
+        };
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
-                s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8_t*>(kp + kt * 32 * LDK + 16 * j), q[j], s[kt], 0, 0, 0);
+        for (int j = 0; j < AHEAD; ++j) read_k(j);
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[j % AHEAD][kt], q[j], s[kt], 0, 0, 0);
+            if (j + AHEAD < NS) read_k(j + AHEAD);
+        }
+        // in this order: the compiler would read each operand right before its product
+        __builtin_amdgcn_sched_group_barrier(0x100, 2 * AHEAD, 0);  // LDS reads
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);  // products
+            if (j + AHEAD < NS) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
+        const u16* vp = Vs + (4 * hf + ((lane & 15) >> 2)) * LDV + (lane & 16) + 4 * (lane & 3);
+        bf16x8_t vf[2][NDT];
+        auto read_v = [&](int g) {  // V^T of 16 keys
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) vf[g & 1][dt] = join8(read_tr4(vp + 16 * g * LDV + 32 * dt), read_tr4(vp + (16 * g + 8) * LDV + 32 * dt));
+            asm volatile("" ::: "memory");
+        };
+        read_v(0);
         // s[kt][i] = key kb + 32 kt + 8 (i / 4) + 4 hf + i % 4 of this lane's row
         const bool whole = kb + KB - 1 <= wp0 && !(a.window && kb <= wp1 - a.window) && kb + KB <= t.s1 && !hole;
         if (!whole) {
@@ -513,21 +537,18 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
         }
         const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+        for (int g = 0; g < 4; ++g) {
+            float p[8];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                float p[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][8 * u + e], sc, -ref));
-                    l += p[e];
-                }
-                const bf16x8_t ph = __builtin_bit_cast(bf16x8_t, u32x4_t{pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]), pack_bf16(p[4], p[5]), pack_bf16(p[6], p[7])});
-                const u16* vrow = Vs + (32 * kt + 16 * u + 4 * hf + ((lane & 15) >> 2)) * LDV + (lane & 16) + 4 * (lane & 3);
-#pragma unroll
-                for (int dt = 0; dt < NDT; ++dt)
-                    acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(join8(read_tr4(vrow + 32 * dt), read_tr4(vrow + 8 * LDV + 32 * dt)), ph, acc[dt], 0, 0, 0);
+            for (int e = 0; e < 8; ++e) {
+                p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g >> 1][8 * (g & 1) + e], sc, -ref));
+                l += p[e];
             }
+            const bf16x8_t ph = __builtin_bit_cast(bf16x8_t, u32x4_t{pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]), pack_bf16(p[4], p[5]), pack_bf16(p[6], p[7])});
+            if (g < 3) read_v(g + 1);
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[g & 1][dt], ph, acc[dt], 0, 0, 0);
+        }
     }
 
     l = fold_halves(l, fadd2);
