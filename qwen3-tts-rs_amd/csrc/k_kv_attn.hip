@@ -327,12 +327,12 @@ __global__ __launch_bounds__(256, RG == 1 ? 3 : 2) void kv_attend_few_kernel(KvA
 // ------------------------------------------------------------------------------------------------------ 128 rows a tile
 // Prompts and chunks: bound by the matrix and vector instructions, so 128 rows share one staging (and conversion) of 64 keys: four waves of 32
 // rows, the K and V images in LDS, the next block of keys travelling in registers, two blocks of threads a CU (three at d = 64) that fill each
-// other's waits.  Measured (d = 128): equal tiles, 1024 of them, 870 TFLOP/s in bf16, 930 in e4m3 (half the bytes from L2); a large library product
-// 1257.  Prompts of 4096 and 2912 tokens 160 us = 650 TFLOP/s: the longest tile walks 64 blocks of keys at 2.5 us; 509 new tokens behind 3 x 15013
-// e4m3 keys 380 us = 765.  Counters of the prompts: matrix pipe busy 35 % of the CUs' time, vector pipe 37 %, LDS 26 % without a
-// conflict: neither is full, a wave's chain S -> softmax -> P V is what waits.  Tried, not faster: S of the next block issued before the softmax of
+// other's waits.  Measured (d = 128): equal tiles, 1024 of them, 975 TFLOP/s in bf16, 1020 in e4m3 (half the bytes from L2); a large library product
+// 1257.  Prompts of 4096 and 2912 tokens 133 us = 775 TFLOP/s: the longest tile walks 64 blocks of keys at 2.1 us; 509 new tokens behind 3 x 15013
+// e4m3 keys 359 us = 808.  Counters of the prompts before the reads went ahead and the priorities: matrix pipe busy 35 % of the CUs' time, vector
+// pipe 37 %, LDS 26 % without a conflict: none was full, a wave's chain S -> softmax -> P V was what waited.  Tried, not faster: S of the next block issued before the softmax of
 // this one over double images; 256 rows with eight waves (prompts 7 % faster, chunks and windows slower); longest tiles at a higher wave
-// priority; blocks of keys dealt evenly to the CUs (the tiles of a head no longer walk in step and miss the L2).
+// priority from end to end; blocks of keys dealt evenly to the CUs (the tiles of a head no longer walk in step and miss the L2).
 template <int FMT, int D>
 __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) {
     constexpr bool Q8 = FMT != KV_BF16;
@@ -476,6 +476,9 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[kt][i] = 0.f;
+        // A wave at its products goes before one that stages or waits, one further on before one at its start: the two blocks of a CU, which
+        // start in step, come apart (prompts 155 -> 133 us, equal tiles 3 to 6 % faster; at d = 64 no gain, the window's case 5 % slower).
+        if constexpr (D == 128) __builtin_amdgcn_s_setprio(1);
         const u16* kp = Ks + r * LDK + 8 * hf;
         constexpr int AHEAD = 3;
         bf16x8_t kf[AHEAD][2];
@@ -536,6 +539,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
             m = mn;
         }
         const float ref = m == -INFINITY ? 0.f : m;
+        if constexpr (D == 128) __builtin_amdgcn_s_setprio(2);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             float p[8];
@@ -549,6 +553,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
 #pragma unroll
             for (int dt = 0; dt < NDT; ++dt) acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[g & 1][dt], ph, acc[dt], 0, 0, 0);
         }
+        if constexpr (D == 128) __builtin_amdgcn_s_setprio(0);
     }
 
     l = fold_halves(l, fadd2);

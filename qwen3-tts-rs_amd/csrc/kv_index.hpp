@@ -87,8 +87,8 @@ inline KvAttendPlan kv_attend_plan(const KvLayer& kv, const KvBatch& b, int nh, 
     KvAttendPlan p{};
     const long rows = (long)b.max_new * (nh / kv.nkv);
     // Every tile walks, and in 8 bits converts, its keys by itself; a 128-row tile is slow to start and partly empty.  Measured in us (d = 128) with
-    // tiles of 16 / 32 / 128 rows: 16 rows of 128 x 8192 int8 keys 53 61 79, bf16 107 107 103, of 512 x 2000 int8 47 56 75, of 8 x 300 bf16
-    // 12 13 13; 20 rows 87 64 79, 130 114 108, 103 59 75, 12 13 13; 48 rows 152 116 91, 260 133 111, 140 107 86, 12 14 14.
+    // tiles of 16 / 32 / 128 rows: 16 rows of 128 x 8192 int8 keys 56 65 75, bf16 109 109 106, of 512 x 2000 int8 49 57 67, of 8 x 300 bf16
+    // 12 13 13; 20 rows 90 65 71, 132 114 109, 100 59 67, 12 13 12; 48 rows 152 116 79, 255 134 111, 138 111 74, 12 14 13.
     p.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 128;
     p.tiles = (int)std::min<long>((rows + p.tile_rows - 1) / p.tile_rows, 65536);  // the grid's y: callers refuse more than 65535
     // keys the tile with the most of them can see
@@ -105,10 +105,10 @@ inline KvAttendPlan kv_attend_plan(const KvLayer& kv, const KvBatch& b, int nh, 
     } else {
         // The parts' number with the least time by this account: a CU walks 64 keys with one, two (three at head_dim 64) resident blocks in
         // the microseconds below; a block costs two walks on top; parts cost a launch and their partial results, written and read at 5 TB/s.
-        // Measured with 1 / 2 / 4 / 8 parts (d = 128, bf16): 64 tiles of 8192 keys 198 111 64 56 us, 256 of them 202 176 180 200, 384 of them
-        // 285 282 283 313, 512 of them 335 354 371 421; 256 tiles of up to 512 keys 21 33 36 36; 512 of up to 4096 114 113 124 134 (the keys a
+        // Measured with 1 / 2 / 4 / 8 parts (d = 128, bf16): 64 tiles of 8192 keys 187 105 62 53 us, 256 of them 195 164 179 198, 384 of them
+        // 261 283 273 307, 512 of them 302 326 348 403; 256 tiles of up to 512 keys 20 33 35 36; 512 of up to 4096 114 104 122 135 (the keys a
         // tile of a prompt sees depend on its place, the account takes the most for all).
-        static constexpr float WALK[2][4] = {{0.f, 1.2f, 1.6f, 2.4f}, {0.f, 1.65f, 2.7f, 0.f}};
+        static constexpr float WALK[2][4] = {{0.f, 1.2f, 1.6f, 2.4f}, {0.f, 1.5f, 2.45f, 0.f}};
         const int most = kv.d == 64 ? 3 : 2;  // resident blocks of a CU
         const float* walk = WALK[kv.d == 64 ? 0 : 1];
         float best = 0.f;
