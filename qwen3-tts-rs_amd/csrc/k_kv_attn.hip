@@ -13,7 +13,8 @@
 // 2^-8 relative per term, as the output itself is afterwards; l is summed from the unrounded f32 values.
 // Key ranges are cut into parts where a call has too few tiles to fill the GPU (kv_attend_plan); a second launch joins their (m, l, O).
 // A masked key may hold anything: its score is replaced, and its V row meets the products as zero.  Where some rows of a tile see a key
-// and others do not, a non-finite V element is taken out of the products and added to the rows that see it one by one.
+// and others do not, a non-finite V element is taken out of the products and added to the rows that see it one by one.  (An infinity whose
+// weight f32 takes for zero, below 2^-126 of the row's largest, may come out as NaN: 0 * infinity.)
 #include "kv_device.hpp"
 
 #include <algorithm>
@@ -344,7 +345,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
     constexpr int KPW = 64 / PPR, NP = KB / (4 * KPW);  // keys a wave stages at once, passes per block of keys
     __shared__ __attribute__((aligned(16))) u16 Ks[KB * LDK];
     __shared__ __attribute__((aligned(16))) u16 Vs[KB * LDV];
-    __shared__ int sh_bad;
+    __shared__ int sh_bad;  // a V element that some rows see and others do not was not finite
 
     const int pair = blockIdx.x;
     if (pair >= a.b.n_seq * a.kv.nkv) return;
@@ -409,12 +410,11 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
         load(t.s0);
         pv = kv_page16(a, t, t.s0 + KB + 16 * (lane & 3));
     }
-    if (threadIdx.x == 0) sh_bad = -1;
+    if (threadIdx.x == 0) sh_bad = 0;
     for (int kb = t.s0; kb < t.s1; kb += KB) {
         const bool mixed = kb + KB - 1 > t.p0 || (a.window && kb <= t.p1 - a.window);
         const bool edge = mixed || kb < t.k_begin || kb + KB > t.s1 || holes;
         __syncthreads();  // every wave is done with the previous image
-        bool bad = false;
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
             const int k0 = (n * 4 + wave) * KPW;
@@ -435,39 +435,19 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
 #pragma unroll
                 for (int h = 0; h < (Q8 ? 2 : 1); ++h) {
                     w[h] = keep(w[h], in);
-                    bad |= mixed && bf16x8_bad(w[h]);
+                    if (mixed && bf16x8_bad(w[h])) {
+                        sh_bad = 1;  // read behind the loop, and so behind a barrier
+                        w[h] = bf16x8_clean(w[h]);
+                    }
                 }
             }
 #pragma unroll
             for (int h = 0; h < (Q8 ? 2 : 1); ++h) *reinterpret_cast<u32x4_t*>(Vs + key * LDV + pc * EPP + 8 * h) = w[h];
         }
-        if (bad) sh_bad = kb;
         hole = holes;
         load(kb + KB);  // behind the part: page 0, not used
         pv = kv_page16(a, t, kb + 2 * KB + 16 * (lane & 3));
         __syncthreads();
-        if (mixed && sh_bad == kb) {
-            if (wlive) {
-                for (int j = 0; j < KB; ++j) {
-                    const int key = kb + j;
-                    if (key >= klo && key <= pos) {
-#pragma unroll
-                        for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) acc[dt][i] += bad_only(Vs[j * LDV + 32 * dt + 8 * (i >> 2) + 4 * hf + (i & 3)]);
-                    }
-                }
-            }
-            __syncthreads();
-#pragma unroll
-            for (int n = 0; n < NP; ++n)
-#pragma unroll
-                for (int h = 0; h < (Q8 ? 2 : 1); ++h) {
-                    u32x4_t* p = reinterpret_cast<u32x4_t*>(Vs + ((n * 4 + wave) * KPW + krow) * LDV + pc * EPP + 8 * h);
-                    *p = bf16x8_clean(*p);
-                }
-            __syncthreads();
-        }
         // wave-uniform: no row of this wave sees the block
         if (!wlive || kb > wp1 || (a.window && kb + KB <= wp0 - a.window + 1)) continue;
 
@@ -554,6 +534,37 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
             for (int dt = 0; dt < NDT; ++dt) acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[g & 1][dt], ph, acc[dt], 0, 0, 0);
         }
         if constexpr (D == 128) __builtin_amdgcn_s_setprio(0);
+    }
+
+    // What was taken out of the products, added to the rows that see it: here, behind the last scaling of acc, and not in the loop, where a
+    // factor of 0 (a row's first block, a maximum that rises by 2^7 or more) would make NaN of an infinity.
+    if (t.s0 < t.s1 && sh_bad) {
+        for (int key = t.s0; key < t.s1; ++key) {
+            const int kb = key & ~(KB - 1);
+            if (!(kb + KB - 1 > t.p0 || (a.window && kb <= t.p1 - a.window)) || key < klo || key > pos) continue;
+            const int page = kv_page(a.kv, t.s.row, key);
+            if (page < 0) continue;
+            const size_t vr = kv_row(a.kv, page, 1, t.g, key);
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const size_t at = vr * D + 32 * dt + 2 * i + 4 * hf;
+                    float v[4];
+                    if constexpr (Q8) {
+                        kv_decode4<FMT>(*reinterpret_cast<const unsigned*>(a.kv.codes + at), kv_scale(a.kv.scales[at / KV_BLOCK]), v);
+                    } else {
+                        const uint2 w = *reinterpret_cast<const uint2*>((const u16*)a.kv.codes + at);
+                        v[0] = __uint_as_float(w.x << 16);
+                        v[1] = __uint_as_float(w.x & 0xffff0000u);
+                        v[2] = __uint_as_float(w.y << 16);
+                        v[3] = __uint_as_float(w.y & 0xffff0000u);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!__builtin_isfinite(v[e])) acc[dt][i + e] += v[e];
+                }
+        }
     }
 
     l = fold_halves(l, fadd2);

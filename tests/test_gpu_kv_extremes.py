@@ -1,0 +1,73 @@
+"""Attention over the key/value cache (KVCache.attend) where values are infinite: the kernels of few and of many rows against plain
+implementations in 64 bits (kv_reference.py)."""
+import math
+
+import pytest
+import torch
+
+from kv_reference import attend as ref_attend, held
+from qwen3_tts_rs_amd import KVCache
+from test_gpu_kv_cache import bounds, rand, table_of
+
+pytestmark = pytest.mark.gpu
+
+
+def cache_with(k, v, fmt="bf16", page=64):
+    """One sequence of the given keys and values on shuffled pages: the cache and a function (new, ctx) -> batch."""
+    n, kv, d = k.shape
+    table, pages = table_of([n], page)
+    cache = KVCache(pages=pages, kv_heads=kv, head_dim=d, format=fmt, page_tokens=page)
+    cache.write(0, cache.batch([n], [n], table), k, v)
+    return cache, lambda new, ctx: cache.batch([new], [ctx], table)
+
+
+# --------------------------------------------------------------------------------------------------------------- infinities
+def check_infinite(out, q, k, v, scale, window=0):
+    """Rows that see an infinity: the formula's infinities and NaN (of both signs: NaN); every other element within its bound."""
+    e = ref_attend(q, k.double(), v.double(), scale, window)
+    got = out.double().cpu()
+    assert torch.equal(got.isnan(), e.isnan())
+    assert torch.equal(got.isinf(), e.isinf()) and torch.equal(got[e.isinf()], e[e.isinf()])
+    # the bound of the finite elements: without the infinities, none of which a row with a finite element of that column sees
+    clean = v.double().cpu().nan_to_num(0, 0, 0)
+    tol = bounds(q, k.double(), clean, scale, window, e.nan_to_num(0, 0, 0))
+    assert ((got - e).abs() <= tol)[e.isfinite()].all()
+
+
+@pytest.mark.parametrize("window", [0, 20])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,new", [(1, 9), (2, 70), (2, 200), (5, 300)])
+def test_infinite_values_from_the_first_key_on(heads, new, dim, window):
+    """A prompt from nothing: infinities among the first keys a tile sees, where no maximum is known yet, and in every block after."""
+    k, v, q = rand((new, 1, dim), 1), rand((new, 1, dim), 2), rand((new, heads, dim), 3)
+    for i, at in enumerate(range(0, new, 13)):
+        v[at, 0, (3 * i) % dim] = math.inf if i % 3 else -math.inf
+    v[3, 0, 5], v[5, 0, 5] = math.inf, -math.inf  # both signs: NaN for the rows that see both
+    cache, batch = cache_with(k, v)
+    check_infinite(cache.attend(0, batch(new, new), q, window=window), q, k, v, dim ** -0.5, window)
+
+
+@pytest.mark.parametrize("ctx", [700, 1040, 1100, 1290, 1601, 2070])
+def test_infinite_values_where_a_part_begins(ctx):
+    """Parts of the key range that begin among the chunk's own keys, which some of its rows see and others do not."""
+    d, new, heads = 128, 128, 1
+    k, v, q = rand((ctx, 1, d), 1), rand((ctx, 1, d), 2), rand((new, heads, d), 3)
+    for i, back in enumerate((1, 20, 41, 62, 83, 104, 125)):
+        v[ctx - back, 0, 7 * i] = math.inf
+    v[10, 0, 100] = -math.inf  # seen by all
+    cache, batch = cache_with(k, v)
+    b = batch(new, ctx)
+    check_infinite(cache.attend(0, b, q), q, k, v, d ** -0.5)
+
+
+@pytest.mark.parametrize("heads,new", [(1, 30), (1, 130), (4, 130)])
+def test_infinite_values_beside_a_maximum_that_jumps(heads, new):
+    """The first 64 keys score about 320 below the others (2^-460 of their weights): the infinity stands beside the higher ones."""
+    d, ctx = 64, 130
+    k, v, q = rand((ctx, 1, d), 1), rand((ctx, 1, d), 2), rand((new, heads, d), 3)
+    q[:, :, 0] = 16
+    k[:, :, 0] = 0
+    k[:64, :, 0] = -160
+    v[100, 0, 9], v[117, 0, 30] = math.inf, -math.inf
+    cache, batch = cache_with(k, v)
+    check_infinite(cache.attend(0, batch(new, ctx), q), q, k, v, d ** -0.5)
