@@ -510,7 +510,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
         // The reference m of the exponentials need not be the maximum, only near it: it moves when a row's maximum has left it by more than
         // 2^8 (p and l stay far from overflow, their relative precision is the same).  Moved at every new maximum, which some row of 32 has in
         // most blocks, acc's scaling was a fifth of the vector instructions.
-        if (__any(mx > m + 8.f)) {
+        if (__any(mx - m > 8.f)) {
             const float mn = fmaxf(m, mx);
             const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
             l *= alpha;
@@ -518,14 +518,30 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
             for (int dt = 0; dt < NDT; ++dt) acc[dt] *= alpha;
             m = mn;
         }
-        const float ref = m == -INFINITY ? 0.f : m;
+        // m is a rounded product; the exponents below are s sc - m with one rounding at the end.  The rounding that m had is a factor common to
+        // the row, at most 2^(1/16) while m is below 2^20.  Above, it would drive weights out of f32's range (by 2^64 at 2^30): there the
+        // products are rounded as m was, so that the largest weight is at most 2^8 again.
+        float ref = m == -INFINITY ? 0.f : m, fac = sc;
+        const bool far = fabsf(ref) >= 1048576.f;
+        if (__any(far)) {
+#pragma clang fp contract(off)  // two roundings
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float x = s[kt][i] * sc;
+                    s[kt][i] = far ? x - ref : s[kt][i];
+                }
+            fac = far ? 1.f : sc;
+            ref = far ? 0.f : ref;
+        }
         if constexpr (D == 128) __builtin_amdgcn_s_setprio(2);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             float p[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g >> 1][8 * (g & 1) + e], sc, -ref));
+                p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g >> 1][8 * (g & 1) + e], fac, -ref));
                 l += p[e];
             }
             const bf16x8_t ph = __builtin_bit_cast(bf16x8_t, u32x4_t{pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]), pack_bf16(p[4], p[5]), pack_bf16(p[6], p[7])});

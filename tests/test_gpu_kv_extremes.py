@@ -1,5 +1,5 @@
-"""Attention over the key/value cache (KVCache.attend) where values are infinite: the kernels of few and of many rows against plain
-implementations in 64 bits (kv_reference.py)."""
+"""Attention over the key/value cache (KVCache.attend) where values are infinite or scores are large: the kernels of few and of many
+rows against plain implementations in 64 bits (kv_reference.py)."""
 import math
 
 import pytest
@@ -71,3 +71,43 @@ def test_infinite_values_beside_a_maximum_that_jumps(heads, new):
     v[100, 0, 9], v[117, 0, 30] = math.inf, -math.inf
     cache, batch = cache_with(k, v)
     check_infinite(cache.attend(0, batch(new, ctx), q), q, k, v, d ** -0.5)
+# ------------------------------------------------------------------------------------------------------------- large scores
+@pytest.mark.parametrize("top", [1e7, 1e9, 1e10, 1e12, 1e20, 1e30, 1e37])
+@pytest.mark.parametrize("heads,new,ctx", [(1, 1, 150), (1, 5, 150), (8, 4, 150), (40, 5, 150), (2, 150, 150), (3, 60, 900), (1, 40, 3000)])
+def test_large_finite_scores(heads, new, ctx, top):
+    """Scores of up to `top`: one product of two bf16 numbers each, exact in f32.  Two of them that differ do so by 2^-8 of the
+    larger, 2^15 and more, so that every weight but the largest is zero (or the same, where scores are the same) and the f32
+    rounding of a score does not count: what is left of the bound is the rounding of weights and output and the sums.  Every third
+    token's scores are ordinary ones, below 8."""
+    d = 64
+    k, v = torch.zeros(ctx, 1, d), rand((ctx, 1, d), 2)
+    k[:, 0, 0] = torch.randint(-255, 256, (ctx,), generator=torch.Generator().manual_seed(5)).float() / 256
+    k = k.to(torch.bfloat16).cuda()
+    q = rand((new, heads, d), 3)
+    small = torch.arange(new) % 3 == 2
+    # scale 2^40 at the top end: raw scores stay below the largest f32
+    scale = 2.0 ** -3 if top < 1e20 else 2.0 ** 40
+    q[:, :, 0] = 2.0 ** math.floor(math.log2(top / scale))
+    q[small, :, 0] = 8.0 / scale
+    cache, batch = cache_with(k, v)
+    out = cache.attend(0, batch(new, ctx), q, scale=scale).double().cpu()
+    e = ref_attend(q, k.double(), v.double(), scale)
+    a = ref_attend(q, k.double(), v.double().abs(), scale)
+    assert e.isfinite().all()
+    # z = 8 in the bound of the ordinary tokens (bounds() in test_gpu_kv_cache.py)
+    tol = 1.01 * (2.0 ** -8 * e.abs() + (2.0 ** -8 + 2 * (d + 4) * 2.0 ** -24 * 8 + (ctx + 100) * 2.0 ** -23) * a)
+    assert ((out - e).abs() <= tol).all(), float(((out - e).abs() / tol).nan_to_num(1e9).max())
+
+
+@pytest.mark.parametrize("heads", [1, 40])
+def test_scores_that_overflow_as_products_with_the_scale(heads):
+    """Finite q k whose product with the scale is not: +infinity, so the row is NaN as with an infinite q k, whatever the kernel."""
+    d, ctx = 64, 70
+    k, v, q = torch.zeros(ctx, 1, d, dtype=torch.bfloat16, device="cuda"), rand((ctx, 1, d), 2), rand((2, heads, d), 3)
+    q[:, :, 0] = 2.0 ** 60
+    k[5, 0, 0] = 2.0 ** 20
+    cache, batch = cache_with(k, v)
+    b = batch(2, ctx)
+    assert cache.attend(0, b, q, scale=2.0 ** 50).isnan().all()
+    out = cache.attend(0, b, q, scale=2.0 ** 40)  # 2^120: the one key
+    assert torch.equal(out, v[5].expand(2, heads, d))
