@@ -509,9 +509,10 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
         mx = fold_halves(mx, fmax2) * sc;
         // The reference m of the exponentials need not be the maximum, only near it: it moves when a row's maximum has left it by more than
         // 2^8 (p and l stay far from overflow, their relative precision is the same).  Moved at every new maximum, which some row of 32 has in
-        // most blocks, acc's scaling was a fifth of the vector instructions.
+        // most blocks, acc's scaling was a fifth of the vector instructions.  Each row decides for itself: a row's result does not depend on what
+        // shares its wave.
         if (__any(mx - m > 8.f)) {
-            const float mn = fmaxf(m, mx);
+            const float mn = mx - m > 8.f ? mx : m;
             const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
             l *= alpha;
 #pragma unroll

@@ -1,5 +1,5 @@
-"""Attention over the key/value cache (KVCache.attend) where values are infinite or scores are large: the kernels of few and of many
-rows against plain implementations in 64 bits (kv_reference.py)."""
+"""Attention over the key/value cache (KVCache.attend) where values are infinite, scores are large, or a token's neighbours in the
+call change: the kernels of few and of many rows against plain implementations in 64 bits (kv_reference.py)."""
 import math
 
 import pytest
@@ -7,7 +7,7 @@ import torch
 
 from kv_reference import attend as ref_attend, held
 from qwen3_tts_rs_amd import KVCache
-from test_gpu_kv_cache import bounds, rand, table_of
+from test_gpu_kv_cache import bounds, rand, table_of, workspace
 
 pytestmark = pytest.mark.gpu
 
@@ -111,3 +111,20 @@ def test_scores_that_overflow_as_products_with_the_scale(heads):
     assert cache.attend(0, b, q, scale=2.0 ** 50).isnan().all()
     out = cache.attend(0, b, q, scale=2.0 ** 40)  # 2^120: the one key
     assert torch.equal(out, v[5].expand(2, heads, d))
+
+
+# ------------------------------------------------------------------------------------------------------ neighbours in a call
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3", "int8"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_prompt_in_two_parts_gives_the_same(dim, fmt, window):
+    """The last tokens of a prompt get bit for bit what they get when the first ones come in a call before: a row's result depends on
+    its own scores alone, not on which rows share its tile (one part of the keys in all calls)."""
+    n, heads = 300, 4
+    k, v, q = rand((n, 2, dim), 1), rand((n, 2, dim), 2), rand((n, heads, dim), 3, scale=4.0)
+    cache, batch = cache_with(k, v, fmt)
+    assert workspace(cache, batch(n, n), heads, window) == 0
+    whole = cache.attend(0, batch(n, n), q, window=window)
+    for cut in (1, 7, 64, 100, 203, 259):
+        assert torch.equal(cache.attend(0, batch(n - cut, n), q[cut:], window=window), whole[cut:]), cut
+        assert torch.equal(cache.attend(0, batch(cut, cut), q[:cut], window=window), whole[:cut]) or 2 * cut <= 32, cut
