@@ -56,7 +56,8 @@ int qtts_model_load_tensor(qtts_model* m, const char* hf_key, const void* data, 
 int qtts_model_load_tensor_device(qtts_model* m, const char* hf_key, const void* data, int src_dtype,
                                   const int64_t* shape, int rank);
 /* Holds the talker's key/value cache in the format QTTS_KV_E4M3 or QTTS_KV_INT8 (defined with qtts_kv_open below): half the
- * memory and half the bytes a decode step reads per key.  QTTS_KV_BF16, the default, keeps it in the model's dtype.  bf16 models
+ * memory and half the bytes a decode step reads per key.  QTTS_KV_BF16, the default, keeps it in the model's dtype.  Keys and values
+ * alone are rounded to the format: queries and attention weights keep the 16 bits they have over the model's own cache.  bf16 models
  * only.  Takes effect with the next generate call on the handle; sessions opened later start with the model's choice. */
 int qtts_model_set_kv_cache(qtts_model* m, int format);
 /* Checks that every tensor the configs require is present, builds fused weights, RoPE tables and the

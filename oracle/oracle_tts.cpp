@@ -229,7 +229,7 @@ static void hold8(float* x, int d, float top) {
 // -------------------------------------------------------------------------- decoder layer
 // Diagnostic only (0 in every parity check): rounds the named intermediate tensors to bf16 so that the storage precision of
 // a reduced-precision implementation can be priced tensor by tensor.  bit 0: normed layer inputs, bit 1: keys / values,
-// bit 2: attention output, bit 3: MLP activation; bits 8-18: tensors of the codec decoder (oracle_codec.cpp).
+// bit 2: attention output, bit 3: MLP activation, bit 4: queries, bit 5: attention probabilities; bits 8-18: tensors of the codec decoder (oracle_codec.cpp).
 static int g_round_probe = 0;
 void set_round_probe(int mask) { g_round_probe = mask; }
 void probe_round(float* x, size_t n, int bit) {
@@ -274,6 +274,7 @@ void decoder_layer(const Weights& w, const std::string& p, const AttnShape& a, c
     }
     probe_round(k.data(), k.size(), 1);
     probe_round(v.data(), v.size(), 1);
+    probe_round(q.data(), q.size(), 4);
     // KV append (kv_cache.rs:38-42)
     if (cache.len + T > cache.cap) throw std::runtime_error("oracle: kv cache overflow");
     for (int t = 0; t < T; ++t)
@@ -304,6 +305,7 @@ void decoder_layer(const Weights& w, const std::string& p, const AttnShape& a, c
                 sc[(size_t)j] = sv;
             }
             softmax_inplace(sc.data(), kv_len);
+            probe_round(sc.data(), (size_t)kv_len, 5);
             float* o = &attn[((size_t)t * nh + h) * d];
             for (int i = 0; i < d; ++i) o[i] = 0.f;
             for (int j = 0; j < kv_len; ++j) {

@@ -166,7 +166,6 @@ void launch_kv_read(hipStream_t st, int dtype, const KvMoveArgs& a) { launch_kv_
 struct KvPostArgs {
     QkvPostArgs p;
     KvLayer kv;
-    bf16_t* q;
 };
 __device__ __forceinline__ unsigned half_wave_max(unsigned v) {
 #pragma unroll
@@ -216,9 +215,9 @@ __global__ __launch_bounds__(64) void kv_qkv_post_kernel(KvPostArgs args) {
     }
     if (!act) return;  // head_dim 64: the upper half of the wave
     if (is_q) {
-        bf16_t* q = args.q + (long)m * a.nh * d + (long)hi * d;
-        q[i] = from_f32<bf16_t>(x1);
-        q[i + half] = from_f32<bf16_t>(x2);
+        float* q = a.q_out + (long)m * a.nh * d + (long)hi * d;
+        q[i] = x1;
+        q[i + half] = x2;
     } else {
         const int g = is_k ? hi - a.nh : hi - a.nh - a.nkv;
         const int page = kv_page(args.kv, t.row, t.pos);
@@ -228,10 +227,10 @@ __global__ __launch_bounds__(64) void kv_qkv_post_kernel(KvPostArgs args) {
         kv_store_block<FMT>(args.kv, row, i + half, x2);
     }
 }
-void launch_kv_qkv_post(hipStream_t st, const QkvPostArgs& a, const KvLayer& kv, void* q_bf16) {
+void launch_kv_qkv_post(hipStream_t st, const QkvPostArgs& a, const KvLayer& kv) {
     QTTS_CHECK(a.d == 64 || a.d == 128, ERR_SHAPE, "kv qkv_post: head_dim must be 64 or 128");
     QTTS_CHECK(a.M >= 1 && a.nh >= 1 && a.nkv >= 1 && kv.d == a.d && kv.nkv == a.nkv && a.toks, ERR_SHAPE, "kv qkv_post: bad shape");
-    const KvPostArgs args{a, kv, (bf16_t*)q_bf16};
+    const KvPostArgs args{a, kv};
     const dim3 grid((unsigned)a.M, (unsigned)(a.nh + 2 * a.nkv));
     if (kv.format == KV_E4M3) kv_launch(kv_qkv_post_kernel<KV_E4M3>, grid, dim3(64), st, args);
     else if (kv.format == KV_INT8) kv_launch(kv_qkv_post_kernel<KV_INT8>, grid, dim3(64), st, args);

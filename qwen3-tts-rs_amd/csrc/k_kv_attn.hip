@@ -11,6 +11,8 @@
 //                 which the lanes hold them; V^T comes out of a row-major LDS image by transposing reads.
 // Rounding: K, V and Q enter exactly (bf16, or codes times a power of two).  P is rounded to bf16 for the second product, at most
 // 2^-8 relative per term, as the output itself is afterwards; l is summed from the unrounded f32 values.
+// WIDE (the talker over its 8-bit cache): f32 queries and P enter as a bf16 value plus a bf16 remainder, two products each, as over its
+// 16-bit cache, so that of the formats' choice nothing but K and V is rounded; the output has a remainder plane of its own.
 // Key ranges are cut into parts where a call has too few tiles to fill the GPU (kv_attend_plan); a second launch joins their (m, l, O).
 // A masked key may hold anything: its score is replaced, and its V row meets the products as zero.  Where some rows of a tile see a key
 // and others do not, a non-finite V element is taken out of the products and added to the rows that see it one by one.  (An infinity whose
@@ -50,6 +52,20 @@ __device__ __forceinline__ u32x4_t bf16x8_clean(u32x4_t w) {
     return u32x4_t{bf16_pair_clean(w.x), bf16_pair_clean(w.y), bf16_pair_clean(w.z), bf16_pair_clean(w.w)};
 }
 __device__ __forceinline__ u32x4_t keep(u32x4_t w, bool in) { return in ? w : u32x4_t{0u, 0u, 0u, 0u}; }
+// eight f32 as bf16 plus bf16 remainder
+__device__ __forceinline__ bf16x8_t pack8(const float* f) {
+    return __builtin_bit_cast(bf16x8_t, u32x4_t{pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7])});
+}
+__device__ __forceinline__ bf16x8_t rest8(const float* f, bf16x8_t hi) {
+    const u32x4_t w = __builtin_bit_cast(u32x4_t, hi);
+    float r[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        r[2 * i] = f[2 * i] - __uint_as_float(w[i] << 16);
+        r[2 * i + 1] = f[2 * i + 1] - __uint_as_float(w[i] & 0xffff0000u);
+    }
+    return pack8(r);
+}
 // value added to a row that sees a V element: the element if it is not finite (it was taken out of the products), else nothing
 __device__ __forceinline__ float bad_only(u16 b) { return (b & 0x7f80u) == 0x7f80u ? bf16_bits_to_f32(b) : 0.f; }
 
@@ -60,7 +76,7 @@ __device__ __forceinline__ float bad_only(u16 b) { return (b & 0x7f80u) == 0x7f8
 // one walk (and one conversion of 8-bit keys) instead of walking twice.  Measured (d = 128): 12 x 30011 int8 keys of 8 kv heads 124 us with the join = 4.8 TB/s
 // (a large copy: 4.89), 64 x 500 e4m3 keys 13 us = 3.9 TB/s, 32 x 2047 int8 keys with five tokens 27 us (+ 5 us of joining), 113 keys of one sequence 6 us,
 // of which all is latency.  Four waves a SIMD instead of three spilled registers and were slower.
-template <int FMT, int D, int RG>
+template <int FMT, int D, int RG, bool WIDE>
 __global__ __launch_bounds__(256, RG == 1 ? 3 : 2) void kv_attend_few_kernel(KvAttendArgs a) {
     constexpr bool Q8 = FMT != KV_BF16;
     constexpr int TR = 16 * RG;                        // a lane holds scores of RG rows, 16 apart
@@ -85,7 +101,7 @@ __global__ __launch_bounds__(256, RG == 1 ? 3 : 2) void kv_attend_few_kernel(KvA
     // this lane's rows: their key ranges and queries
     int pos[RG], klo[RG];
     bool has[RG];
-    bf16x8_t q[RG][NJ];
+    bf16x8_t q[RG][NJ], ql[RG][WIDE ? NJ : 1];
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg) {
         const int row = t.row0 + 16 * rg + r;
@@ -93,11 +109,18 @@ __global__ __launch_bounds__(256, RG == 1 ? 3 : 2) void kv_attend_few_kernel(KvA
         const int rr = has[rg] ? row : t.row0, tok = rr / t.G, head = t.g * t.G + rr - tok * t.G;
         pos[rg] = t.s.ctx - t.s.n + tok;
         klo[rg] = has[rg] ? (a.window ? pos[rg] - a.window + 1 : 0) : 0x7fffffff;
-        const u16* qp = (const u16*)a.q + (long)(t.s.t0 + tok) * a.q_token_stride + (long)head * a.q_head_stride;
+        const long qat = (long)(t.s.t0 + tok) * a.q_token_stride + (long)head * a.q_head_stride;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             const int d0 = Q8 ? 64 * (j >> 1) + 16 * gq + 8 * (j & 1) : 32 * j + 8 * gq;
-            q[rg][j] = *reinterpret_cast<const bf16x8_t*>(qp + d0);
+            if constexpr (WIDE) {
+                float f[8];
+                load8((const float*)a.q + qat + d0, f);
+                q[rg][j] = pack8(f);
+                ql[rg][j] = rest8(f, q[rg][j]);
+            } else {
+                q[rg][j] = *reinterpret_cast<const bf16x8_t*>((const u16*)a.q + qat + d0);
+            }
         }
     }
 
@@ -196,6 +219,10 @@ __global__ __launch_bounds__(256, RG == 1 ? 3 : 2) void kv_attend_few_kernel(KvA
                     for (int rg = 0; rg < RG; ++rg) {
                         s[rg][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, q[rg][2 * j], s[rg][kt], 0, 0, 0);
                         s[rg][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, q[rg][2 * j + 1], s[rg][kt], 0, 0, 0);
+                        if constexpr (WIDE) {
+                            s[rg][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, ql[rg][2 * j], s[rg][kt], 0, 0, 0);
+                            s[rg][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, ql[rg][2 * j + 1], s[rg][kt], 0, 0, 0);
+                        }
                     }
                 }
             } else {
@@ -212,7 +239,7 @@ __global__ __launch_bounds__(256, RG == 1 ? 3 : 2) void kv_attend_few_kernel(KvA
         load(kb + 128, pg);  // behind the part: page 0, not used
         pv = kv_page16(a, t, kb + 256 + 16 * (lane & 1));
 
-        bf16x8_t ph[RG];
+        bf16x8_t ph[RG], pr[RG];  // pr: the remainders
 #pragma unroll
         for (int rg = 0; rg < RG; ++rg) {
             float p[8], mx = -INFINITY;
@@ -234,7 +261,8 @@ __global__ __launch_bounds__(256, RG == 1 ? 3 : 2) void kv_attend_few_kernel(KvA
                 ps += p[e];
             }
             l[rg] = l[rg] * alpha + ps;
-            ph[rg] = __builtin_bit_cast(bf16x8_t, u32x4_t{pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]), pack_bf16(p[4], p[5]), pack_bf16(p[6], p[7])});
+            ph[rg] = pack8(p);
+            if constexpr (WIDE) pr[rg] = rest8(p, ph[rg]);
 #pragma unroll
             for (int dt = 0; dt < NDT; ++dt) acc[rg][dt] *= alpha;
         }
@@ -266,7 +294,10 @@ __global__ __launch_bounds__(256, RG == 1 ? 3 : 2) void kv_attend_few_kernel(KvA
         for (int dt = 0; dt < NDT; ++dt) {
             const bf16x8_t vt = join8(read_tr4(vrow + 16 * dt), read_tr4(vrow + 16 * LDV + 16 * dt));
 #pragma unroll
-            for (int rg = 0; rg < RG; ++rg) acc[rg][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt, ph[rg], acc[rg][dt], 0, 0, 0);
+            for (int rg = 0; rg < RG; ++rg) {
+                acc[rg][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt, ph[rg], acc[rg][dt], 0, 0, 0);
+                if constexpr (WIDE) acc[rg][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt, pr[rg], acc[rg][dt], 0, 0, 0);
+            }
         }
         __builtin_amdgcn_wave_barrier();
     }
@@ -334,7 +365,7 @@ __global__ __launch_bounds__(256, RG == 1 ? 3 : 2) void kv_attend_few_kernel(KvA
 // pipe 37 %, LDS 26 % without a conflict: none was full, a wave's chain S -> softmax -> P V was what waited.  Tried, not faster: S of the next block issued before the softmax of
 // this one over double images; 256 rows with eight waves (prompts 7 % faster, chunks and windows slower); longest tiles at a higher wave
 // priority from end to end; blocks of keys dealt evenly to the CUs (the tiles of a head no longer walk in step and miss the L2).
-template <int FMT, int D>
+template <int FMT, int D, bool WIDE>
 __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) {
     constexpr bool Q8 = FMT != KV_BF16;
     constexpr int KB = 64;
@@ -365,11 +396,20 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
     const int tok = rr / t.G, head = t.g * t.G + rr - tok * t.G;
     const int pos = first + tok;
     const int klo = has ? (a.window ? pos - a.window + 1 : 0) : 0x7fffffff;
-    bf16x8_t q[NS];
+    bf16x8_t q[NS], ql[WIDE ? NS : 1];
     {
-        const u16* qp = (const u16*)a.q + (long)(t.s.t0 + tok) * a.q_token_stride + (long)head * a.q_head_stride + 8 * hf;
+        const long qat = (long)(t.s.t0 + tok) * a.q_token_stride + (long)head * a.q_head_stride + 8 * hf;
 #pragma unroll
-        for (int j = 0; j < NS; ++j) q[j] = *reinterpret_cast<const bf16x8_t*>(qp + 16 * j);
+        for (int j = 0; j < NS; ++j) {
+            if constexpr (WIDE) {
+                float f[8];
+                load8((const float*)a.q + qat + 16 * j, f);
+                q[j] = pack8(f);
+                ql[j] = rest8(f, q[j]);
+            } else {
+                q[j] = *reinterpret_cast<const bf16x8_t*>((const u16*)a.q + qat + 16 * j);
+            }
+        }
     }
     f32x16_t acc[NDT];
 #pragma unroll
@@ -472,13 +512,17 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
         for (int j = 0; j < NS; ++j) {
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[j % AHEAD][kt], q[j], s[kt], 0, 0, 0);
+            if constexpr (WIDE) {
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[j % AHEAD][kt], ql[j], s[kt], 0, 0, 0);
+            }
             if (j + AHEAD < NS) read_k(j + AHEAD);
         }
         // in this order: the compiler would read each operand right before its product
         __builtin_amdgcn_sched_group_barrier(0x100, 2 * AHEAD, 0);  // LDS reads
 #pragma unroll
         for (int j = 0; j < NS; ++j) {
-            __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);  // products
+            __builtin_amdgcn_sched_group_barrier(0x8, WIDE ? 4 : 2, 0);  // products
             if (j + AHEAD < NS) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
         }
         const u16* vp = Vs + (4 * hf + ((lane & 15) >> 2)) * LDV + (lane & 16) + 4 * (lane & 3);
@@ -545,10 +589,15 @@ __global__ __launch_bounds__(256, 2) void kv_attend_tile_kernel(KvAttendArgs a) 
                 p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g >> 1][8 * (g & 1) + e], fac, -ref));
                 l += p[e];
             }
-            const bf16x8_t ph = __builtin_bit_cast(bf16x8_t, u32x4_t{pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]), pack_bf16(p[4], p[5]), pack_bf16(p[6], p[7])});
+            const bf16x8_t ph = pack8(p);
             if (g < 3) read_v(g + 1);
 #pragma unroll
             for (int dt = 0; dt < NDT; ++dt) acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[g & 1][dt], ph, acc[dt], 0, 0, 0);
+            if constexpr (WIDE) {
+                const bf16x8_t pr = rest8(p, ph);
+#pragma unroll
+                for (int dt = 0; dt < NDT; ++dt) acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[g & 1][dt], pr, acc[dt], 0, 0, 0);
+            }
         }
         if constexpr (D == 128) __builtin_amdgcn_s_setprio(0);
     }
@@ -718,28 +767,38 @@ void launch_kv_attend(hipStream_t st, KvAttendArgs a, const KvAttendPlan& p) {
     // pairs vary fastest and are padded to the number of XCDs: all tiles and parts of a pair run on one XCD and share its L2
     const dim3 grid((pairs + 7) / 8 * 8, (unsigned)p.tiles, (unsigned)p.splits);
     const dim3 join(pairs * (unsigned)p.tiles, p.tile_rows == 128 ? (unsigned)a.kv.d / 8u : (unsigned)p.tile_rows / 4u);
-#define QTTS_KV_ATTEND(FMT, DD)                                                                         \
-    if (a.kv.format == FMT && a.kv.d == DD) {                                                           \
+#define QTTS_KV_ATTEND(FMT, DD, WIDE)                                                                   \
+    if (a.kv.format == FMT && a.kv.d == DD && a.wide == WIDE) {                                         \
         if (p.tile_rows == 16) {                                                                        \
-            kv_launch(kv_attend_few_kernel<FMT, DD, 1>, grid, dim3(256), st, a);                        \
+            kv_launch(kv_attend_few_kernel<FMT, DD, 1, WIDE>, grid, dim3(256), st, a);                  \
             if (p.splits > 1) kv_launch(kv_attend_join_few_kernel<DD, 16>, join, dim3(256), st, a);     \
-        } else if (p.tile_rows == 32) {                                                                 \
-            kv_launch(kv_attend_few_kernel<FMT, DD, 2>, grid, dim3(256), st, a);                        \
-            if (p.splits > 1) kv_launch(kv_attend_join_few_kernel<DD, 32>, join, dim3(256), st, a);     \
-        } else {                                                                                        \
-            kv_launch(kv_attend_tile_kernel<FMT, DD>, grid, dim3(256), st, a);                          \
-            if (p.splits > 1) kv_launch(kv_attend_join_tile_kernel<DD>, join, dim3(256), st, a);        \
+            return;                                                                                     \
         }                                                                                               \
-        return;                                                                                         \
+        if constexpr (!WIDE) {                                                                          \
+            if (p.tile_rows == 32) {                                                                    \
+                kv_launch(kv_attend_few_kernel<FMT, DD, 2, WIDE>, grid, dim3(256), st, a);              \
+                if (p.splits > 1) kv_launch(kv_attend_join_few_kernel<DD, 32>, join, dim3(256), st, a); \
+                return;                                                                                 \
+            }                                                                                           \
+        }                                                                                               \
+        if (p.tile_rows == 128) {                                                                       \
+            kv_launch(kv_attend_tile_kernel<FMT, DD, WIDE>, grid, dim3(256), st, a);                    \
+            if (p.splits > 1) kv_launch(kv_attend_join_tile_kernel<DD>, join, dim3(256), st, a);        \
+            return;                                                                                     \
+        }                                                                                               \
     }
-    QTTS_KV_ATTEND(KV_BF16, 64)
-    QTTS_KV_ATTEND(KV_E4M3, 64)
-    QTTS_KV_ATTEND(KV_INT8, 64)
-    QTTS_KV_ATTEND(KV_BF16, 128)
-    QTTS_KV_ATTEND(KV_E4M3, 128)
-    QTTS_KV_ATTEND(KV_INT8, 128)
+    QTTS_KV_ATTEND(KV_BF16, 64, false)
+    QTTS_KV_ATTEND(KV_E4M3, 64, false)
+    QTTS_KV_ATTEND(KV_INT8, 64, false)
+    QTTS_KV_ATTEND(KV_BF16, 128, false)
+    QTTS_KV_ATTEND(KV_E4M3, 128, false)
+    QTTS_KV_ATTEND(KV_INT8, 128, false)
+    QTTS_KV_ATTEND(KV_E4M3, 64, true)
+    QTTS_KV_ATTEND(KV_INT8, 64, true)
+    QTTS_KV_ATTEND(KV_E4M3, 128, true)
+    QTTS_KV_ATTEND(KV_INT8, 128, true)
 #undef QTTS_KV_ATTEND
-    throw Error(ERR_SHAPE, "kv cache: head_dim must be 64 or 128");
+    throw Error(ERR_SHAPE, "kv attend: no kernel for this head_dim, format and tile");
 }
 
 }  // namespace qtts

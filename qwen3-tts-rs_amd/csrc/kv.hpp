@@ -50,14 +50,14 @@ struct KvMoveArgs {         // write: k, v -> cache; read: cache -> k, v
 void launch_kv_write(hipStream_t st, int dtype, const KvMoveArgs& a);
 void launch_kv_read(hipStream_t st, int dtype, const KvMoveArgs& a);
 
-// q|k|v projection rows -> per-head RMSNorm, RoPE, queries in bf16 [M][nh d] and keys / values into the cache (the 8-bit
-// counterpart of launch_qkv_post; a.toks name row and position of every token, a.q_out is not written)
-void launch_kv_qkv_post(hipStream_t st, const QkvPostArgs& a, const KvLayer& kv, void* q_bf16);
+// q|k|v projection rows -> per-head RMSNorm, RoPE, queries in f32 and keys / values into the cache (the 8-bit counterpart of
+// launch_qkv_post; a.toks name row and position of every token)
+void launch_kv_qkv_post(hipStream_t st, const QkvPostArgs& a, const KvLayer& kv);
 
 struct KvAttendArgs {
     KvLayer kv;
     KvBatch b;
-    const void* q;          // bf16
+    const void* q;          // bf16; f32 if wide
     long q_token_stride, q_head_stride;
     void* out;              // bf16
     long out_token_stride, out_head_stride;
@@ -66,6 +66,7 @@ struct KvAttendArgs {
     float scale;
     int window;             // a token sees at most this many keys, its own included; 0 = all
     float* ws;              // partial results when plan.splits > 1
+    bool wide;              // f32 queries, which enter as two bf16 pieces as the probabilities do (8-bit formats, tiles of 16 or 128 rows: the talker)
     // filled from the plan
     int tiles, splits, split_len;
 };

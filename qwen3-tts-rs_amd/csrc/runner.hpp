@@ -236,13 +236,13 @@ struct Runner {
         else
             launch_attention(st, dt, g.q.as<float>(), toks, kv, kv_layer, M, c.nh, scale, g.attn.p, lo_attn);
     }
-    // the same over the 8-bit cache, prompts and decode steps alike; the f32 query buffer takes the queries in bf16
+    // the same over the 8-bit cache, prompts and decode steps alike
     void attention_kv8(const StackCfg& c, const QkvPostArgs& qa, int kv_layer, float scale) {
         KvAttendArgs a{};
         a.kv = kv8->layer(kv_layer);
-        launch_kv_qkv_post(st, qa, a.kv, g.q.p);
+        launch_kv_qkv_post(st, qa, a.kv);
         a.b = kv8->batch;
-        a.q = g.q.p; a.q_token_stride = (long)c.nh * c.d; a.q_head_stride = c.d;
+        a.q = g.q.p; a.wide = true; a.q_token_stride = (long)c.nh * c.d; a.q_head_stride = c.d;
         a.out = g.attn.p; a.out_token_stride = (long)c.nh * c.d; a.out_head_stride = c.d; a.out_lo = lo_attn;
         a.nh = c.nh; a.scale = scale; a.window = c.window >= a.b.max_ctx ? 0 : c.window;
         a.ws = kv8->ws;
