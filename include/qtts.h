@@ -305,14 +305,15 @@ typedef struct {
     const int32_t* page_table; /* [n_seq][max_pages] */
 } qtts_kv_batch;
 /* k and v rows [n_tokens][kv_heads][head_dim] with strides in elements; the head_dim elements of a row are contiguous, pointers and
- * strides (of dimensions longer than one) are multiples of 16 bytes. */
+ * strides (of dimensions longer than one) are multiples of 16 bytes.  Rows that are read into do not overlap: k and v in one buffer (halves of
+ * a packed row, say) have the same strides. */
 typedef struct {
     void *k, *v;
     int dtype;                /* QTTS_F32 or QTTS_BF16 */
     int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
 } qtts_kv_rows;
 /* q and out rows [n_tokens][n_heads][head_dim], bf16; strides as above.  out may be q, with the same strides; otherwise the two do not
- * overlap. */
+ * overlap (views of one buffer that lie between each other's rows have the same strides).  What does overlap is refused. */
 typedef struct {
     const void* q;
     void* out;

@@ -87,7 +87,7 @@ static KvBatch check_batch(const KvCache& k, int layer, const qtts_kv_batch& b) 
 }
 
 // `n` rows of `heads` x d elements of `es` bytes: 16-byte accesses; an output's rows may not overlap
-static void check_rows(const void* p, int64_t n, int64_t heads, int64_t d, int64_t ts, int64_t hs, int64_t es, bool output, const char* what) {
+static KvRowsAt check_rows(const void* p, int64_t n, int64_t heads, int64_t d, int64_t ts, int64_t hs, int64_t es, bool output, const char* what) {
     const std::string name(what);
     QTTS_CHECK(p, ERR_BAD_ARG, name + ": null tensor");
     if (n <= 1) ts = 0;  // the stride of a single token or head is not used
@@ -95,8 +95,9 @@ static void check_rows(const void* p, int64_t n, int64_t heads, int64_t d, int64
     QTTS_CHECK(((uintptr_t)p & 15) == 0 && ts * es % 16 == 0 && hs * es % 16 == 0, ERR_BAD_ARG, name + ": pointer and strides must be multiples of 16 bytes");
     QTTS_CHECK(ts >= 0 && hs >= 0 && ts < (int64_t)1 << 40 && hs < (int64_t)1 << 40, ERR_BAD_ARG, name + ": stride out of range");
     if (output)
-        QTTS_CHECK((heads == 1 || hs >= d) && (n <= 1 || ts >= d) && (ts >= (heads - 1) * hs + d || hs >= (n - 1) * ts + d || n <= 1 || heads == 1), ERR_BAD_ARG,
+        QTTS_CHECK((heads == 1 || hs >= d) && (n <= 1 || ts >= d) && (ts >= (heads - 1) * hs + d || (__int128)hs >= (__int128)(n - 1) * ts + d || n <= 1 || heads == 1), ERR_BAD_ARG,
                    name + ": rows of an output overlap");
+    return KvRowsAt{(int64_t)(uintptr_t)p, ts * es, hs * es};
 }
 
 static void kv_move(const KvCache& k, int layer, const qtts_kv_batch& b, const qtts_kv_rows& r, hipStream_t st, bool write) {
@@ -105,9 +106,10 @@ static void kv_move(const KvCache& k, int layer, const qtts_kv_batch& b, const q
     QTTS_CHECK(r.dtype == F32 || r.dtype == BF16, ERR_BAD_ARG, "kv cache: keys and values must be QTTS_F32 or QTTS_BF16");
     if (b.n_seq == 0 || b.n_tokens == 0 || b.max_new == 0) return;
     const int64_t es = (int64_t)dtype_size(r.dtype);
-    check_rows(r.k, b.n_tokens, k.nkv, k.d, r.k_token_stride, r.k_head_stride, es, !write, "kv cache: k");
-    check_rows(r.v, b.n_tokens, k.nkv, k.d, r.v_token_stride, r.v_head_stride, es, !write, "kv cache: v");
+    const KvRowsAt kr = check_rows(r.k, b.n_tokens, k.nkv, k.d, r.k_token_stride, r.k_head_stride, es, !write, "kv cache: k");
+    const KvRowsAt vr = check_rows(r.v, b.n_tokens, k.nkv, k.d, r.v_token_stride, r.v_head_stride, es, !write, "kv cache: v");
     QTTS_CHECK(write || r.k != r.v, ERR_BAD_ARG, "kv cache: k and v are read into one tensor");
+    QTTS_CHECK(write || !kv_rows_overlap(kr, vr, b.n_tokens, k.nkv, k.d * es), ERR_BAD_ARG, "kv cache: k and v are read into rows that overlap");
     a.kv = k.layer(layer, b);
     a.k_in = r.k; a.v_in = r.v; a.k_out = r.k; a.v_out = r.v;
     a.k_token_stride = r.k_token_stride; a.k_head_stride = r.k_head_stride;
@@ -142,8 +144,11 @@ void kv_attend(const KvCache& k, int layer, const qtts_kv_batch& b, const qtts_k
         return;
     }
     const KvAttendPlan p = check_plan(k, b, a.b, r.n_heads, r.window);
-    check_rows(r.q, b.n_tokens, r.n_heads, k.d, r.q_token_stride, r.q_head_stride, 2, false, "kv attend: q");
-    check_rows(r.out, b.n_tokens, r.n_heads, k.d, r.out_token_stride, r.out_head_stride, 2, true, "kv attend: out");
+    const KvRowsAt qr = check_rows(r.q, b.n_tokens, r.n_heads, k.d, r.q_token_stride, r.q_head_stride, 2, false, "kv attend: q");
+    const KvRowsAt outr = check_rows(r.out, b.n_tokens, r.n_heads, k.d, r.out_token_stride, r.out_head_stride, 2, true, "kv attend: out");
+    const bool in_place = qr.at == outr.at && qr.token == outr.token && qr.head == outr.head;
+    QTTS_CHECK(in_place || !kv_rows_overlap(qr, outr, b.n_tokens, r.n_heads, k.d * 2), ERR_BAD_ARG,
+               "kv attend: out overlaps q without being it, with the same strides");
     QTTS_CHECK(p.ws_bytes == 0 || (r.workspace && ((uintptr_t)r.workspace & 15) == 0 && r.workspace_bytes >= (int64_t)p.ws_bytes), ERR_BAD_ARG,
                "kv attend: the workspace is smaller than qtts_kv_attend_workspace asks for, or not aligned to 16 bytes");
     a.kv = k.layer(layer, b);

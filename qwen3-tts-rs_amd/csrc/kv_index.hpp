@@ -4,6 +4,7 @@
 #include "kv.hpp"
 
 #include <algorithm>
+#include <cstdint>
 
 #define QTTS_KV_HD __host__ __device__ __forceinline__
 
@@ -83,6 +84,33 @@ QTTS_KV_HD int kv_page16(const KvAttendArgs& a, const KvTile& t, int key) {
 }
 
 // ---- host
+// Rows [n][heads] of `row` bytes, strides in bytes (0 for a dimension of one).  The two of a question have the same n, heads and row.
+struct KvRowsAt {
+    int64_t at, token, head;
+};
+// Do the rows of a and b share a byte?  With equal strides exactly; with others, rows between each other's first and last byte count as
+// shared (row i of one may then meet row j of the other in more ways than are worth telling apart).
+inline bool kv_rows_overlap(const KvRowsAt& a, const KvRowsAt& b, int64_t n, int64_t heads, int64_t row) {
+    typedef __int128 wide;  // strides and counts are the caller's: their product may pass 64 bits
+    const auto end = [&](const KvRowsAt& r) { return (wide)r.at + (wide)(n - 1) * r.token + (wide)(heads - 1) * r.head + row; };
+    if (b.at >= end(a) || a.at >= end(b)) return false;
+    if (a.token != b.token || a.head != b.head) return true;
+    // the difference of two rows' addresses is i token + j head with |i| < n, |j| < heads: for each j the two nearest i
+    const bool swap = heads > n;  // walk the shorter dimension
+    const wide walk = swap ? a.token : a.head, step = swap ? a.head : a.token, delta = (wide)b.at - a.at;
+    const int64_t nw = swap ? n : heads, ns = swap ? heads : n;
+    for (int64_t j = 1 - nw; j < nw; ++j) {
+        const wide r = delta - j * walk;
+        wide i = step ? r / step : 0;
+        if (step && r < 0 && i * step != r) --i;  // floor
+        for (int k = 0; k < 2; ++k, ++i) {
+            const wide c = i < 1 - ns ? 1 - ns : (i > ns - 1 ? ns - 1 : i), x = r - c * step;
+            if (x < row && -x < row) return true;
+        }
+    }
+    return false;
+}
+
 inline KvAttendPlan kv_attend_plan(const KvLayer& kv, const KvBatch& b, int nh, int window) {
     KvAttendPlan p{};
     const long rows = (long)b.max_new * (nh / kv.nkv);
