@@ -56,6 +56,7 @@ class KVCache:
         import torch
         self._torch = torch
         self._f32, self._bf16 = torch.float32, torch.bfloat16
+        self._forward_ad = torch.autograd.forward_ad
         # the stream's handle without a Stream object around it (2 us of a call's 10) where torch has that
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         self._stream = (lambda: raw(int(device))) if raw else (lambda: torch.cuda.current_stream(self.device).cuda_stream)
@@ -132,6 +133,8 @@ class KVCache:
             raise QttsError(-1, f"{what}: the elements of a head must be contiguous")
         if t.requires_grad and self._torch.is_grad_enabled():
             raise QttsError(-1, f"{what}: inference only, the tensor requires a gradient")
+        if self._forward_ad._current_level >= 0 and self._forward_ad.unpack_dual(t).tangent is not None:
+            raise QttsError(-1, f"{what}: inference only, the tensor has a tangent")
 
     def _move(self, call, layer, batch, k, v):
         r = _lib.KvRows(k.data_ptr(), v.data_ptr(), QTTS_F32 if k.dtype == self._f32 else QTTS_BF16, k.stride(0), k.stride(1), v.stride(0),

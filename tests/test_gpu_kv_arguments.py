@@ -55,3 +55,19 @@ def test_output_that_overlaps_the_queries(heads):
         keep = q.clone()
         cache.attend(0, b, q, out=out)
         check_attend(out, keep, k, v, [n], [n], "bf16", d ** -0.5)
+
+
+def test_tensors_with_a_tangent():
+    """Forward-mode differentiation: refused, as a tensor that requires a gradient is, instead of a result that has lost its tangent."""
+    import torch.autograd.forward_ad as fwad
+    n, d = 5, 64
+    cache, b, k, v = _cache(n, 1, d)
+    q = rand((n, 2, d), 3)
+    with fwad.dual_level():
+        for call in (lambda: cache.attend(0, b, fwad.make_dual(q, q)), lambda: cache.attend(0, b, q, out=fwad.make_dual(q.clone(), q)),
+                     lambda: cache.write(0, b, fwad.make_dual(k, k), v), lambda: cache.write(0, b, k, fwad.make_dual(v, v)),
+                     lambda: cache.read(0, b, out=(fwad.make_dual(k.clone(), k), v.clone()))):
+            with pytest.raises(QttsError, match="tangent"):
+                call()
+        out = cache.attend(0, b, q)  # without one, inside the level
+    check_attend(out, q, k, v, [n], [n], "bf16", d ** -0.5)
