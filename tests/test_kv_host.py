@@ -7,7 +7,7 @@ import pytest
 from conftest import ROOT
 
 
-@pytest.mark.parametrize("program", ["kv_overlap"])
+@pytest.mark.parametrize("program", ["kv_overlap", "kv_parts"])
 def test_host_program(tmp_path, program):
     exe = str(tmp_path / program)
     r = subprocess.run(["/opt/rocm/bin/hipcc", "-std=c++17", "-O1", "-x", "hip", "--cuda-host-only", "-I", os.path.join(ROOT, "qwen3-tts-rs_amd", "csrc"),
