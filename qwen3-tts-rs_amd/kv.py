@@ -104,7 +104,7 @@ class KVCache:
         if len(new) != len(ctx) or any(n < 0 or n > c for n, c in zip(new, ctx)):
             raise QttsError(-1, "KVCache.batch: every sequence needs 0 <= new <= ctx")
         if not isinstance(page_table, torch.Tensor):
-            page_table = torch.tensor(page_table, dtype=torch.int32).reshape(len(new), -1).to(self.device)
+            page_table = torch.tensor(page_table, dtype=torch.int32).reshape(len(new), -1 if new else 0).to(self.device)
         start = [0]
         for n in new:
             start.append(start[-1] + n)

@@ -71,3 +71,14 @@ def test_tensors_with_a_tangent():
                 call()
         out = cache.attend(0, b, q)  # without one, inside the level
     check_attend(out, q, k, v, [n], [n], "bf16", d ** -0.5)
+
+
+def test_a_step_of_no_sequences_from_host_numbers():
+    """A serving loop whose sequences have all ended passes empty lists."""
+    cache, _, k, _ = _cache(5, 1, 64)
+    b = cache.batch([], [], [])
+    none = k[:0]
+    cache.write(0, b, none, none)
+    assert cache.attend(0, b, none).shape == (0, 1, 64) and cache.read(0, b)[0].shape == (0, 1, 64)
+    b = cache.batch([0, 0], [5, 0], [[0], [-1]])
+    assert cache.attend(0, b, none).shape == (0, 1, 64)
