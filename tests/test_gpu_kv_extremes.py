@@ -36,7 +36,7 @@ def check_infinite(out, q, k, v, scale, window=0):
 
 @pytest.mark.parametrize("window", [0, 20])
 @pytest.mark.parametrize("dim", [64, 128])
-@pytest.mark.parametrize("heads,new", [(1, 9), (2, 70), (2, 200), (5, 300)])
+@pytest.mark.parametrize("heads,new", [(1, 9), (3, 9), (2, 70), (2, 200), (5, 300)])
 def test_infinite_values_from_the_first_key_on(heads, new, dim, window):
     """A prompt from nothing: infinities among the first keys a tile sees, where no maximum is known yet, and in every block after."""
     k, v, q = rand((new, 1, dim), 1), rand((new, 1, dim), 2), rand((new, heads, dim), 3)
@@ -47,10 +47,11 @@ def test_infinite_values_from_the_first_key_on(heads, new, dim, window):
     check_infinite(cache.attend(0, batch(new, new), q, window=window), q, k, v, dim ** -0.5, window)
 
 
+@pytest.mark.parametrize("new", [128, 127, 30, 15])
 @pytest.mark.parametrize("ctx", [700, 1040, 1100, 1290, 1601, 2070])
-def test_infinite_values_where_a_part_begins(ctx):
+def test_infinite_values_where_a_part_begins(ctx, new):
     """Parts of the key range that begin among the chunk's own keys, which some of its rows see and others do not."""
-    d, new, heads = 128, 128, 1
+    d, heads = 128, 1
     k, v, q = rand((ctx, 1, d), 1), rand((ctx, 1, d), 2), rand((new, heads, d), 3)
     for i, back in enumerate((1, 20, 41, 62, 83, 104, 125)):
         v[ctx - back, 0, 7 * i] = math.inf
@@ -60,7 +61,7 @@ def test_infinite_values_where_a_part_begins(ctx):
     check_infinite(cache.attend(0, b, q), q, k, v, d ** -0.5)
 
 
-@pytest.mark.parametrize("heads,new", [(1, 30), (1, 130), (4, 130)])
+@pytest.mark.parametrize("heads,new", [(1, 16), (1, 30), (1, 130), (4, 130)])
 def test_infinite_values_beside_a_maximum_that_jumps(heads, new):
     """The first 64 keys score about 320 below the others (2^-460 of their weights): the infinity stands beside the higher ones."""
     d, ctx = 64, 130
@@ -73,7 +74,7 @@ def test_infinite_values_beside_a_maximum_that_jumps(heads, new):
     check_infinite(cache.attend(0, batch(new, ctx), q), q, k, v, d ** -0.5)
 # ------------------------------------------------------------------------------------------------------------- large scores
 @pytest.mark.parametrize("top", [1e7, 1e9, 1e10, 1e12, 1e20, 1e30, 1e37])
-@pytest.mark.parametrize("heads,new,ctx", [(1, 1, 150), (1, 5, 150), (8, 4, 150), (40, 5, 150), (2, 150, 150), (3, 60, 900), (1, 40, 3000)])
+@pytest.mark.parametrize("heads,new,ctx", [(1, 1, 150), (1, 5, 150), (8, 4, 150), (40, 5, 150), (2, 150, 150), (3, 60, 900), (1, 1, 3000), (5, 5, 3000), (1, 40, 3000)])
 def test_large_finite_scores(heads, new, ctx, top):
     """Scores of up to `top`: one product of two bf16 numbers each, exact in f32.  Two of them that differ do so by 2^-8 of the
     larger, 2^15 and more, so that every weight but the largest is zero (or the same, where scores are the same) and the f32
