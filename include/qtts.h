@@ -334,11 +334,13 @@ int qtts_kv_write(qtts_kv_cache* kv, int layer, const qtts_kv_batch* batch, cons
 /* Reads the batch's tokens back (the values they are held as); with n = ctx_len whole sequences. */
 int qtts_kv_read(qtts_kv_cache* kv, int layer, const qtts_kv_batch* batch, const qtts_kv_rows* rows, void* stream);
 /* out = softmax(scale q k^T) v of the batch's tokens over the held keys and values: a token at position p sees positions
- * p-window+1 .. p (0 .. p without a window); a row that sees nothing, or whose every score is
- * -infinity, is zero; a score beyond the largest f32 is infinite, and with +infinity among its scores a row is NaN.  The tokens' own keys and values have been written before.  Weighted values are summed in f32 before they are divided
- * by the weights' sum, with weights of at most 2^8: values beyond 2^119 / (number of keys) may come out as infinity.  An infinite value
- * makes the outputs of the rows that see it infinite, NaN with one of the other sign; where its weight is below 2^-126 of the row's
- * largest, it may give NaN (0 * infinity in f32).  The workspace size depends on the batch's host integers only. */
+ * p-window+1 .. p (0 .. p without a window); a row that sees nothing, or whose every score is -infinity, is zero; a score beyond the
+ * largest f32 is infinite, and with +infinity among its scores a row is NaN.  The tokens' own keys and values have been written before.
+ * Scores, weights and sums are f32; for the product with the values a weight is rounded to bf16 (by 2^-8 of it at most).  Weighted
+ * values are summed before they are divided by the weights' sum, with weights of at most 2^8: values beyond 2^119 / (number of keys) may
+ * come out as infinity.  An infinite value makes the outputs of the rows that see it infinite, NaN with one of the other sign; where its
+ * weight is below 2^-126 of the row's largest, it may give NaN (0 * infinity in f32).  The workspace size depends on the batch's host
+ * integers only. */
 int qtts_kv_attend_workspace(qtts_kv_cache* kv, const qtts_kv_batch* batch, int n_heads, int window, int64_t* bytes);
 int qtts_kv_attend(qtts_kv_cache* kv, int layer, const qtts_kv_batch* batch, const qtts_kv_attend_args* args, void* stream);
 

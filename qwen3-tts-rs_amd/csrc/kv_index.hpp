@@ -115,8 +115,8 @@ inline KvAttendPlan kv_attend_plan(const KvLayer& kv, const KvBatch& b, int nh, 
     KvAttendPlan p{};
     const long rows = (long)b.max_new * (nh / kv.nkv);
     // Every tile walks, and in 8 bits converts, its keys by itself; a 128-row tile is slow to start and partly empty.  Measured in us (d = 128) with
-    // tiles of 16 / 32 / 128 rows: 16 rows of 128 x 8192 int8 keys 56 65 75, bf16 109 109 106, of 512 x 2000 int8 49 57 67, of 8 x 300 bf16
-    // 12 13 13; 20 rows 90 65 71, 132 114 109, 100 59 67, 12 13 12; 48 rows 152 116 79, 255 134 111, 138 111 74, 12 14 13.
+    // tiles of 16 / 32 / 128 rows: 16 rows of 128 x 8192 int8 keys 57 64 71, bf16 104 105 101, of 512 x 2000 int8 48 59 65, of 8 x 300 bf16
+    // 11 12 12; 20 rows 91 65 69, 127 106 102, 86 60 64, 12 12 12; 48 rows 152 114 78, 253 123 105, 123 108 72, 12 14 13.
     p.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 128;
     p.tiles = (int)std::min<long>((rows + p.tile_rows - 1) / p.tile_rows, 65536);  // the grid's y: callers refuse more than 65535
     // keys the tile with the most of them can see
@@ -126,16 +126,18 @@ inline KvAttendPlan kv_attend_plan(const KvLayer& kv, const KvBatch& b, int nh, 
     p.splits = 1;
     if (p.tile_rows != 128) {
         // Two blocks a CU fill it, and a part of fewer than 256 keys is mostly start and join.  Measured with targets of 512 / 768 / 1024
-        // blocks: 12 x 30011 int8 keys 124 / 131 / 140 us, 32 x 2047 with five tokens 32.2 / 30.6 / 34.0 us, 7 x 20011 bf16 keys 23.2 / 26.4 /
-        // 26.5 us; parts of at least 512 keys: 24.8 us for the last.
+        // blocks: 12 x 30011 int8 keys 130 / 140 / 147 us, 32 x 2047 with five tokens 34.7 / 33.7 / 36.3 us, 7 x 20011 bf16 keys 23.8 / 26.8 /
+        // 26.9 us; parts of at least 512 keys: 25.5 us for the last.  The grid keeps a pair on one XCD (launch_kv_attend), so with fewer than
+        // eight pairs as many XCDs have these blocks and the others none: 30000 bf16 keys of 1 / 2 / 4 / 8 pairs all take 30 to 34 us.
         const long want = std::max<long>(1, 512 / std::max<long>(units, 1)), most = std::max<long>(1, (keys + 255) / 256);
         p.splits = (int)std::min<long>(std::min(want, most), KV_MAX_PARTS);
     } else {
         // The parts' number with the least time by this account: a CU walks 64 keys with one, two (three at head_dim 64) resident blocks in
         // the microseconds below; a block costs two walks on top; parts cost a launch and their partial results, written and read at 5 TB/s.
-        // Measured with 1 / 2 / 4 / 8 parts (d = 128, bf16): 64 tiles of 8192 keys 187 105 62 53 us, 256 of them 195 164 179 198, 384 of them
-        // 261 283 273 307, 512 of them 302 326 348 403; 256 tiles of up to 512 keys 20 33 35 36; 512 of up to 4096 114 104 122 135 (the keys a
-        // tile of a prompt sees depend on its place, the account takes the most for all).
+        // Measured with 1 / 2 / 4 / 8 parts (d = 128, bf16): 64 tiles of 8192 keys 186 103 66 62 us, 256 of them 233 210 235 279, 384 of them
+        // 325 354 359 416, 512 of them 391 429 481 560; 256 tiles of up to 512 keys 20 32 35 35; 512 of up to 4096 110 101 119 134 (the keys a
+        // tile of a prompt sees depend on its place, the account takes the most for all).  It takes the blocks as spread over all CUs, which
+        // the grid does from eight pairs on: a prompt of 4096 tokens takes 101 / 110 / 114 / 119 us with 1 / 2 / 4 / 8 pairs.
         static constexpr float WALK[2][4] = {{0.f, 1.2f, 1.6f, 2.4f}, {0.f, 1.5f, 2.45f, 0.f}};
         const int most = kv.d == 64 ? 3 : 2;  // resident blocks of a CU
         const float* walk = WALK[kv.d == 64 ? 0 : 1];
