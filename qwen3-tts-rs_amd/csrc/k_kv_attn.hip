@@ -12,7 +12,7 @@
 // Rounding: K, V and Q enter exactly (bf16, or codes times a power of two).  P is rounded to bf16 for the second product, at most
 // 2^-8 relative per term, as the output itself is afterwards; l is summed from the unrounded f32 values.
 // WIDE (the talker over its 8-bit cache): f32 queries and P enter as a bf16 value plus a bf16 remainder, two products each, as over its
-// 16-bit cache, so that of the formats' choice nothing but K and V is rounded; the output has a remainder plane of its own.
+// 16-bit cache, so that choosing 8 bits rounds K and V alone; the output has a remainder plane of its own.
 // Key ranges are cut into parts where a call has too few tiles to fill the GPU (kv_attend_plan); a second launch joins their (m, l, O).
 // A masked key may hold anything: its score is replaced, and its V row meets the products as zero.  Where some rows of a tile see a key
 // and others do not, a non-finite V element is taken out of the products and added to the rows that see it one by one.  (An infinity whose
@@ -75,7 +75,8 @@ __device__ __forceinline__ float bad_only(u16 b) { return (b & 0x7f80u) == 0x7f8
 // each walks every fourth group of 32 keys with the next group's loads in flight, and the four results are joined in LDS.  32 rows share
 // one walk (and one conversion of 8-bit keys) instead of walking twice.  Measured (d = 128): 12 x 30011 int8 keys of 8 kv heads 124 us with the join = 4.8 TB/s
 // (a large copy: 4.89), 64 x 500 e4m3 keys 13 us = 3.9 TB/s, 32 x 2047 int8 keys with five tokens 27 us (+ 5 us of joining), 113 keys of one sequence 6 us,
-// of which all is latency; the talker's step (WIDE, 64 x 51 .. 91 e4m3 keys) 8.2 us, 7.7 without the second pieces.  Four waves a SIMD instead of three spilled registers and were slower.
+// of which all is latency; the talker's step (WIDE, 64 x 51 .. 91 e4m3 keys) 8.2 us, 7.7 without the second pieces.  Four waves a SIMD instead of
+// three spilled registers and were slower.
 template <int FMT, int D, int RG, bool WIDE>
 __global__ __launch_bounds__(256, RG == 1 ? 3 : 2) void kv_attend_few_kernel(KvAttendArgs a) {
     constexpr bool Q8 = FMT != KV_BF16;
@@ -361,8 +362,8 @@ __global__ __launch_bounds__(256, RG == 1 ? 3 : 2) void kv_attend_few_kernel(KvA
 // rows, the K and V images in LDS, the next block of keys travelling in registers, two blocks of threads a CU (three at d = 64) that fill each
 // other's waits.  Measured (d = 128): 512 equal tiles of 8192 keys 847 TFLOP/s in bf16, 953 in e4m3 (half the bytes), 852 in int8 (byte conversions);
 // 1024 of them 814, 892, 822; a large library product 1257.  Prompts of 4096 and 2912 tokens 131 us = 788 TFLOP/s: the longest tile walks 64 blocks of
-// keys at 2 us; 509 new tokens behind 3 x 15013 e4m3 keys 354 us = 820 (the same in int8: 391).  With two pieces (WIDE) the talker's prompts of 64 x 51 tokens take 22 us a
-// layer, 19 without.  Counters of the prompts before the reads went ahead and the priorities: matrix pipe busy 35 % of the CUs' time, vector
+// keys at 2 us; 509 new tokens behind 3 x 15013 e4m3 keys 354 us = 820 (the same in int8: 391).  The talker's prompts of 64 x 51 tokens (WIDE) take 22 us a
+// layer, 19 without the second pieces.  Counters of the prompts before the reads went ahead and the priorities: matrix pipe busy 35 % of the CUs' time, vector
 // pipe 37 %, LDS 26 % without a conflict: none was full, a wave's chain S -> softmax -> P V was what waited.  Tried, not faster: S of the next block issued before the softmax of
 // this one over double images; 256 rows with eight waves (prompts 7 % faster, chunks and windows slower); longest tiles at a higher wave
 // priority from end to end; blocks of keys dealt evenly to the CUs (the tiles of a head no longer walk in step and miss the L2).

@@ -105,3 +105,41 @@ def test_reference_codes_in_the_prompt(bind, golden, fmt, frames, window):
             ref_text_ids=golden["ref_text_ids"], ref_codes=ref, non_streaming=False, trace=True))], yardstick=fmt == "int8")
     finally:
         m.close()
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_many_heads_on_one_kv_head(bind, fmt):
+    """20 query heads share a kv head: a decode step's rows fill more than one tile of 16."""
+    from qwen3_tts_rs_amd import LoaderConfig, Model, round_bf16, synth
+    cfg, _, tmpl = synth.shape_set("T0")
+    cfg["talker_config"].update(num_attention_heads=20, num_key_value_heads=1)
+    m = Model(cfg, None, LoaderConfig(dtype="bf16", kv_cache=fmt))
+    o = bind.Oracle(fast=False)
+    for k, a in synth.iter_weights(synth.talker_keys(cfg), SEED):
+        a = round_bf16(a)
+        m.load_tensor(k, a)
+        o.load_tensor(k, a)
+    m.finalize()
+    o.set_model_config(cfg)
+    try:
+        text = synth.synthetic_text_ids(tmpl, 40, 3)
+        _check(bind, m, fmt, [(_req(text), lambda: o.generate(text, bind.resolve_codec_prefill(cfg, "english", "speaker1"), GREEDY, FRAMES,
+                                                              speaker_token=bind.resolve_speaker_token(cfg, "speaker1"), trace=True))],
+               yardstick=fmt == "int8")
+    finally:
+        m.close()
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_prompts_of_more_than_one_pass(golden, fmt):
+    """Eight prompts of 5000 tokens in all, one of which is cut between two prefill passes: which one depends on the order of the
+    requests, the logits and codes do not."""
+    from qwen3_tts_rs_amd import SamplingConfig, synthetic_model
+    m, _, _, _ = synthetic_model("T0", dtype="bf16", codec=False, kv_cache=fmt)
+    try:
+        reqs = [_icl_request(golden, np.resize(np.roll(golden["ref_codes"], i, 0), (500 + 37 * i, golden["ref_codes"].shape[1]))) for i in range(8)]
+        a = m.generate(reqs, SamplingConfig.cli_greedy(), 4, trace=True)
+        b = m.generate(reqs[::-1], SamplingConfig.cli_greedy(), 4, trace=True)
+        assert np.array_equal(a.logits, b.logits[::-1]) and np.array_equal(a.codes, b.codes[::-1])
+    finally:
+        m.close()
